@@ -51,6 +51,28 @@ def _dev(*tensors):
       raise KernelError("miniinfer_amd kernels run on the GPU only; got a tensor on " + str(t.device))
 
 
+class _on_device_of:
+  """Launches inside run on the device of these tensors (all on one GPU, or an error) and on its current stream, whatever
+  the current device is."""
+
+  def __init__(self, what, *tensors):
+    _dev(*tensors)
+    devices = {t.device.index for t in tensors if t is not None}
+    if len(devices) > 1:
+      raise KernelError(f"{what}: the tensors are on several devices ({sorted(devices)})")
+    self.index = devices.pop()
+
+  def __enter__(self):
+    self.was = torch.cuda.current_device()
+    if self.was != self.index:
+      torch.cuda.set_device(self.index)
+
+  def __exit__(self, *exc):
+    if self.was != self.index:
+      torch.cuda.set_device(self.was)
+    return False
+
+
 def _contig(name, t):
   if t is not None and not t.is_contiguous():
     raise KernelError(f"{name} must be contiguous")
@@ -140,6 +162,21 @@ _SIGS["sampling"] = {
 _SIGS["probes"] = {
   "mi_probe_stream_read": [c_void_p, c_int64, c_void_p, c_void_p],
   "mi_probe_mfma": [c_int, c_int, c_void_p, c_void_p, c_void_p],
+}
+
+_SIGS["linear_attention"] = {
+  "mi_linear_attention_recurrent": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                    c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_float,
+                                    c_void_p],
+}
+
+_SIGS["beam"] = {
+  "mi_beam_select": [c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+  "mi_beam_scratch": [c_int, c_int, c_int, c_int, c_void_p],
+}
+
+_SIGS["rows"] = {
+  "mi_move_rows": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
 }
 
 _libs = {}
@@ -1089,6 +1126,179 @@ def attn_decode_front(qkv: torch.Tensor, nq: int, nkv: int, d: int, out: torch.T
     nq, nkv, k_pages.shape[2], float(scale), int(window), 1 if stream_keys else 0, 1 if wide else 0, _ptr(q_weight),
     _ptr(k_weight),
     float(eps), _ptr(cos_sin), rotary_dim, max_pos, _ptr(positions), _ptr(slots), _stream()))
+
+
+# ----------------------------------------------------------------------------- linear attention
+
+LINEAR_ATTENTION_MAX_D = 256
+
+
+def _linear_attention_args(what, q, k, v, nq, nkv, d, out, state, state_rows, log_decay):
+  if nkv < 1 or nq < nkv or nq % nkv:
+    raise KernelError(f"{what}: {nq} query heads are no multiple of {nkv} kv heads")
+  if d % 8 or not 8 <= d <= LINEAR_ATTENTION_MAX_D:
+    raise KernelError(f"{what}: head size {d} is no multiple of 8 up to {LINEAR_ATTENTION_MAX_D}")
+  dtype_code(q.dtype)
+  T = q.shape[0]
+  for name, t, heads in (("q", q, nq), ("k", k, nkv), ("v", v, nkv), ("out", out, nq)):
+    if t.dim() != 2 or t.shape[0] != T or t.shape[1] < heads * d or (t.shape[1] > 1 and t.stride(1) != 1):
+      raise KernelError(f"{what}: {name} {tuple(t.shape)} does not hold {T} dense rows of {heads} heads of {d}")
+    if T > 1 and abs(t.stride(0)) < heads * d:
+      raise KernelError(f"{what}: rows of {name} overlap (stride {t.stride(0)})")
+    if t.dtype != q.dtype:
+      raise KernelError(f"{what}: q is {q.dtype}, {name} {t.dtype}")
+  if out.shape[1] != nq * d:
+    raise KernelError(f"{what}: out {tuple(out.shape)} is not [{T}, {nq * d}]")
+  if state.dtype != torch.float32 or state.dim() != 4 or tuple(state.shape[1:]) != (nkv, d, d) \
+      or not state[:1].is_contiguous():
+    raise KernelError(f"{what}: states must be float32 [rows, {nkv}, {d}, {d}] with dense rows, got {tuple(state.shape)} {state.dtype}")
+  if state.shape[0] > 1 and (state.stride(0) < nkv * d * d or state.stride(0) % 4):
+    raise KernelError(f"{what}: rows of states {state.stride(0)} elements apart")
+  if state.data_ptr() % 16:
+    raise KernelError(f"{what}: states must start at a multiple of 16 bytes")
+  _i32("state_rows", state_rows)
+  _f32("log_decay", log_decay, nkv)
+  return T
+
+
+def _linear_attention_call(q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay, scale):
+  T = q.shape[0]
+  stride = lambda t: t.stride(0) if T > 1 else t.shape[1]
+  return (dtype_code(q.dtype), _ptr(q), stride(q), _ptr(k), stride(k), _ptr(v), stride(v), _ptr(out), stride(out), _ptr(state),
+          state.stride(0) if state.shape[0] > 1 else nkv * d * d, state.shape[0], _ptr(state_rows), _ptr(cu_q), T,
+          state_rows.numel(), nq, nkv, d, _ptr(log_decay), float(scale))
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int, nkv: int, d: int, out: torch.Tensor,
+                     state: torch.Tensor, state_rows: torch.Tensor, cu_q: torch.Tensor, log_decay: torch.Tensor,
+                     scale: float, max_len: Optional[int] = None) -> torch.Tensor:
+  """Linear attention with a decay for each head over the tokens of several requests, each going on from its state:
+
+      S_t = a S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t,   a = exp(log_decay[kv head])
+
+  q [T, >= nq*d], k, v [T, >= nkv*d] rows (the parts of a fused q|k|v buffer are fine), out [T, nq*d]; nq / nkv query
+  heads share a kv head's state.  state float32 [rows, nkv, d, d] (key dim, value dim) is read at state_rows[b] and left
+  there as it is after request b's last token; requests of one call have rows of their own.  cu_q int32 [B + 1] = first
+  token of each request: a request without tokens leaves its state as it is, rows of `out` that belong to no request are
+  left as they are, and a state row outside the buffer gives rows of NaN.  log_decay float32 [nkv], <= 0 (-inf: a = 0)
+  or positive for a growing state.  max_len: the most tokens of one request if the host knows it (default: T); it only
+  chooses how the work is cut.  float32 and bfloat16; states and sums are 32-bit."""
+  T = _linear_attention_args("linear_attention", q, k, v, nq, nkv, d, out, state, state_rows, log_decay)
+  _i32("cu_q", cu_q)
+  if cu_q.numel() != state_rows.numel() + 1:
+    raise KernelError(f"linear_attention: cu_q has {cu_q.numel()} entries for {state_rows.numel()} requests")
+  with _on_device_of("linear_attention", q, k, v, out, state, state_rows, cu_q, log_decay):
+    lib = _lib("linear_attention")
+    _check(lib, lib.mi_linear_attention_recurrent(*_linear_attention_call(q, k, v, nq, nkv, d, out, state, state_rows, cu_q,
+                                                                          log_decay, scale), _stream()))
+  return out
+
+
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int, nkv: int, d: int, out: torch.Tensor,
+                          state: torch.Tensor, state_rows: torch.Tensor, log_decay: torch.Tensor,
+                          scale: float) -> torch.Tensor:
+  """`linear_attention` of one token for each request: row b of q, k, v and out is request b's token.  Requests may share
+  a state row that nobody reads afterwards (the padding entries of a captured step do)."""
+  T = _linear_attention_args("linear_attention_step", q, k, v, nq, nkv, d, out, state, state_rows, log_decay)
+  if state_rows.numel() != T:
+    raise KernelError(f"linear_attention_step: {state_rows.numel()} state rows for {T} tokens")
+  with _on_device_of("linear_attention_step", q, k, v, out, state, state_rows, log_decay):
+    lib = _lib("linear_attention")
+    _check(lib, lib.mi_linear_attention_recurrent(*_linear_attention_call(q, k, v, nq, nkv, d, out, state, state_rows, None,
+                                                                          log_decay, scale), _stream()))
+  return out
+
+
+# ----------------------------------------------------------------------------- beam search
+
+BEAM_MAX_COUNT = 64
+BEAM_MAX_BEAMS = 64
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_beams: int,
+                count: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+  """The `count` best continuations of every group of `num_beams` beams: of
+
+      scores[b] + logits[b, v] - log sum_u exp(logits[b, u])      b over the group's beams, v over the vocabulary
+
+  the largest, largest first, equal ones by (beam, token).  logits float32 [G * num_beams, V] with dense rows, scores
+  float32 [G * num_beams] (-inf: a beam that does not take part).  Returns (scores float32, beams int32 in
+  0 .. num_beams - 1, tokens int32), each [G, count].  A logit that is NaN counts as -inf; where a row holds +inf, those
+  tokens share its mass; a row of -inf only has no candidate above -inf.  If fewer than `count` candidates are above -inf
+  the rest of the list has score -inf.  Sums of exponentials and the scores that are compared are 64-bit."""
+  if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    raise KernelError("beam_select: logits must be float32 [beams, V] with dense rows")
+  R, V = logits.shape
+  if num_beams < 1 or R % num_beams or V < 1:
+    raise KernelError(f"beam_select: logits {tuple(logits.shape)} are no groups of {num_beams} beams")
+  if R > 1 and logits.stride(0) < V:
+    raise KernelError("beam_select: rows of logits overlap")
+  _f32("scores", scores, R)
+  G = R // num_beams
+  if num_beams > BEAM_MAX_BEAMS or not 1 <= count <= min(BEAM_MAX_COUNT, num_beams * V):
+    raise KernelError(f"beam_select: {count} of {num_beams} beams x {V} tokens; at most {BEAM_MAX_COUNT} candidates of "
+                      f"{BEAM_MAX_BEAMS} beams are taken")
+  with _on_device_of("beam_select", logits, scores):
+    lib = _lib("beam")
+    words = c_int64(0)
+    _check(lib, lib.mi_beam_scratch(G, num_beams, V, count, ctypes.byref(words)))
+    scratch = torch.empty(words.value, dtype=torch.float64, device=logits.device)
+    out_scores = torch.empty((G, count), dtype=torch.float32, device=logits.device)
+    out = torch.empty((2, G, count), dtype=torch.int32, device=logits.device)
+    _check(lib, lib.mi_beam_select(_ptr(logits), logits.stride(0) if R > 1 else V, _ptr(scores), G, num_beams, V, count,
+                                   _ptr(scratch), _ptr(out_scores), _ptr(out[0]), _ptr(out[1]), _stream()))
+  return out_scores, out[0], out[1]
+
+
+# ----------------------------------------------------------------------------- pages and states
+
+MOVE_ROWS_MAX_BUFFERS = 8
+MOVE_ROWS_MAX = 16384        # moves of a call: one workgroup holds a piece of every moved row in its registers
+
+
+def move_rows(buffers, src: torch.Tensor, dst: torch.Tensor) -> None:
+  """In place, in every layer of every buffer: row dst[i] becomes what row src[i] was before the call, for all i as if
+  at once (permutations and cycles are fine; a row may be a source more than once, a destination only once).  buffers: a
+  tensor or up to 8 of them, [layers, rows, ...] with dense rows, of any dtype: a cache group's key and value pages, a
+  group's states.  src, dst: int32 [n] on the device, n up to 16,384; entries outside a buffer's rows move nothing there
+  (pad with -1)."""
+  if isinstance(buffers, torch.Tensor):
+    buffers = [buffers]
+  buffers = list(buffers)
+  if not 1 <= len(buffers) <= MOVE_ROWS_MAX_BUFFERS:
+    raise KernelError(f"move_rows: {len(buffers)} buffers, 1 to {MOVE_ROWS_MAX_BUFFERS} are taken")
+  for t in buffers:
+    if t.dim() < 2:
+      raise KernelError(f"move_rows: a buffer must be [layers, rows, ...], got {tuple(t.shape)}")
+    if not t[:1, :1].is_contiguous():
+      raise KernelError("move_rows: the rows of a buffer must be dense")
+    if t.numel():
+      extent = t[0, 0].numel()
+      for stride, n in sorted((t.stride(i), t.shape[i]) for i in (0, 1) if t.shape[i] > 1):
+        if stride < extent:
+          raise KernelError(f"move_rows: rows or layers of a buffer overlap (strides {t.stride()})")
+        extent += (n - 1) * stride
+  _i32("src", src)
+  _i32("dst", dst)
+  n = src.numel()
+  if dst.numel() != n:
+    raise KernelError(f"move_rows: {n} sources, {dst.numel()} destinations")
+  if n > MOVE_ROWS_MAX:
+    raise KernelError(f"move_rows: {n} moves, at most {MOVE_ROWS_MAX} are taken")
+  with _on_device_of("move_rows", src, dst, *buffers):
+    lib = _lib("rows")
+    live = [t for t in buffers if t.numel()]
+    if n == 0 or not live:
+      return
+    m = len(live)
+    size = [t.element_size() for t in live]
+    row = [t[0, 0].numel() * e for t, e in zip(live, size)]
+    stride1 = [t.stride(1) * e if t.shape[1] > 1 else r for t, e, r in zip(live, size, row)]
+    stride0 = [t.stride(0) * e if t.shape[0] > 1 else r for t, e, r in zip(live, size, row)]
+    i64, i32 = c_int64 * m, c_int * m
+    _check(lib, lib.mi_move_rows(m, (c_void_p * m)(*[_ptr(t) for t in live]), i64(*stride0), i64(*stride1), i64(*row),
+                                 i32(*[t.shape[0] for t in live]), i32(*[t.shape[1] for t in live]), _ptr(src), _ptr(dst), n,
+                                 _stream()))
 
 
 # ----------------------------------------------------------------------------- what the device delivers
