@@ -168,6 +168,8 @@ _SIGS["linear_attention"] = {
   "mi_linear_attention_recurrent": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
                                     c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_float,
                                     c_void_p],
+  "mi_linear_attention": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int,
+                          c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_float, c_int, c_void_p, c_void_p],
 }
 
 _SIGS["beam"] = {
@@ -1169,6 +1171,14 @@ def _linear_attention_call(q, k, v, nq, nkv, d, out, state, state_rows, cu_q, lo
           state_rows.numel(), nq, nkv, d, _ptr(log_decay), float(scale))
 
 
+def linear_attention_segment(num_tokens: int, max_len: int, nkv: int, d: int, units: int = 256) -> int:
+  """Tokens of a segment into which requests are cut, 0 for none: as many as make two workgroups for every compute unit
+  over all tokens, and at least two chunks."""
+  slices = -(-d // 64)
+  tokens = max(128, -(-num_tokens * nkv * slices // (2 * units * 64)) * 64)
+  return tokens if max_len > tokens else 0
+
+
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int, nkv: int, d: int, out: torch.Tensor,
                      state: torch.Tensor, state_rows: torch.Tensor, cu_q: torch.Tensor, log_decay: torch.Tensor,
                      scale: float, max_len: Optional[int] = None) -> torch.Tensor:
@@ -1189,8 +1199,12 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int,
     raise KernelError(f"linear_attention: cu_q has {cu_q.numel()} entries for {state_rows.numel()} requests")
   with _on_device_of("linear_attention", q, k, v, out, state, state_rows, cu_q, log_decay):
     lib = _lib("linear_attention")
-    _check(lib, lib.mi_linear_attention_recurrent(*_linear_attention_call(q, k, v, nq, nkv, d, out, state, state_rows, cu_q,
-                                                                          log_decay, scale), _stream()))
+    segment = linear_attention_segment(T, T if max_len is None else min(max_len, T), nkv, d, compute_units(q.device))
+    work = None
+    if segment:
+      work = torch.empty((T // segment + state_rows.numel()) * nkv * d * d, dtype=torch.float32, device=q.device)
+    _check(lib, lib.mi_linear_attention(*_linear_attention_call(q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay,
+                                                                scale), segment, _ptr(work), _stream()))
   return out
 
 
