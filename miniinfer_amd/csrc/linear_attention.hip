@@ -160,8 +160,8 @@ MI_EXPORT int mi_linear_attention_recurrent(LA_ARGS, hipStream_t stream) {
 //   S'    = a^n S + sum_j a^(n-1-j) k_j v_j^T
 //
 // Every power has an exponent of 0 or more, so nothing overflows however fast a head forgets.  A workgroup owns VS
-// columns of one request's (or segment's) and kv head's state and walks over the chunks; a wave owns 16 NT of the
-// columns and keeps them, [DP, 16 NT] in 32 bits, in registers as the accumulators of the last product.  Products:
+// columns of one request's (or segment's) and kv head's state and walks over the chunks; a wave owns 16 of the
+// columns and keeps them, [DP, 16] in 32 bits, in registers as the accumulators of the last product.  Products:
 //
 //   P^T = K Q^T        by blocks of 16 queries, one to a wave; weighted, masked, through LDS to every wave
 //   O^T = S^T Q^T      S from the accumulators' registers: an accumulator's lanes sit where an operand's do
@@ -178,32 +178,38 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 
+#ifndef LA_C64
+#define LA_C64 64
+#endif
+#ifndef LA_PBUF64
+#define LA_PBUF64 2
+#endif
 #define LA_LDS(T) __attribute__((address_space(3))) T
 
 template <typename T>
-struct Half;      // 4 elements of an operand
+struct Half;      // 4 elements of an operand, and the two halves of 32 elements of the summed axis
 template <>
 struct Half<bf16> {
   typedef s16x4 type;
+  typedef s16x8 pair;
 };
 template <>
 struct Half<float> {
   typedef f32x4 type;
+  typedef f32x8 pair;
 };
 
-__device__ __forceinline__ bf16x8 join(s16x4 a, s16x4 b) {
-  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+__device__ __forceinline__ s16x8 join(s16x4 a, s16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ f32x8 join(f32x4 a, f32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+// acc += A B over 32 elements of the summed axis
+__device__ __forceinline__ void mma(f32x4& acc, s16x8 a, s16x8 b) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
 }
-// acc += A B over two 16-element pieces of the summed axis
-__device__ __forceinline__ void mma(f32x4& acc, s16x4 a0, s16x4 a1, s16x4 b0, s16x4 b1) {
-  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join(a0, a1), join(b0, b1), acc, 0, 0, 0);
-}
-__device__ __forceinline__ void mma(f32x4& acc, f32x4 a0, f32x4 a1, f32x4 b0, f32x4 b1) {
+__device__ __forceinline__ void mma(f32x4& acc, f32x8 a, f32x8 b) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a0[i], b0[i], acc, 0, 0, 0);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a1[i], b1[i], acc, 0, 0, 0);
+  for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
 }
 __device__ __forceinline__ s16x4 to_half(f32x4 x) { return __builtin_bit_cast(s16x4, __builtin_convertvector(x, bf16x4)); }
 __device__ __forceinline__ f32x4 widen(s16x4 h) {
@@ -235,22 +241,26 @@ struct Split<float, PARTS> {
   static constexpr int parts = 1;
 };
 
-// Tiles in LDS are rows of tokens.  A bfloat16 row is padded by 32 bytes and rows 8 .. 15 of every 16 are shifted by
-// another 16: the 8-byte reads of a half (16 rows, 4 groups) and the transposing reads (4 rows of 32 bytes to 16 lanes)
-// then meet every bank once.  32-bit rows are padded by 16 bytes.
+// Tiles in LDS are rows of tokens.  The two halves that a lane takes to a bfloat16 product, columns 4 g .. and
+// 16 + 4 g .. of every 32, lie side by side (column 16 x + 4 g + i of a block at place 8 g + 4 x + i), so that an
+// operand is one 16-byte read; 32-bit columns keep their order.  Rows are padded by 32 bytes: an operand read, which
+// takes 16 bytes to a lane from 16 rows and 4 neighbouring pieces, is served 4 rows x 2 pieces at a time, and these then
+// lie in different banks.
 template <typename T, int COLS>
 struct Tile {
-  static constexpr int stride = COLS * (int)sizeof(T) + (sizeof(T) == 2 ? 32 : 16);
-  static constexpr int shift = sizeof(T) == 2 ? 16 : 0;
+  static constexpr int stride = COLS * (int)sizeof(T) + 32;
+  // of the 4 columns from col on (a multiple of 4)
   static __device__ __forceinline__ int at(int row, int col) {
-    return row * stride + ((row >> 3) & 1) * shift + col * (int)sizeof(T);
+    if (sizeof(T) == 2) return row * stride + (col & ~31) * 2 + (col & 12) * 4 + (col & 16) / 2;
+    return row * stride + col * 4;
   }
-  static constexpr int bytes(int rows) { return rows * stride + 16; }
+  static constexpr int bytes(int rows) { return rows * stride; }
 };
 
-template <typename T>
-__device__ __forceinline__ typename Half<T>::type half_at(const char* p) {
-  return *reinterpret_cast<const typename Half<T>::type*>(p);
+// The halves of columns col .. col + 31 of the lane's row; `p`: where Tile::at puts (row, 4 g).
+__device__ __forceinline__ s16x8 halves_at(const char* p, int col, bf16*) { return *reinterpret_cast<const s16x8*>(p + col * 2); }
+__device__ __forceinline__ f32x8 halves_at(const char* p, int col, float*) {
+  return join(*reinterpret_cast<const f32x4*>(p + col * 4), *reinterpret_cast<const f32x4*>(p + col * 4 + 64));
 }
 
 // Elements [row 4 g .. 4 g + 3] of column l % 16 of a 16 x 16 piece whose first element is at (row0, col0): the lane's
@@ -264,26 +274,70 @@ template <int COLS>
 __device__ __forceinline__ f32x4 half_down(const char* tile, int row0, int col0, int lane, float*) {
   f32x4 r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const float*>(tile + Tile<float, COLS>::at(row0 + lane / 16 * 4 + i, col0 + lane % 16));
+  for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const float*>(tile + (row0 + lane / 16 * 4 + i) * Tile<float, COLS>::stride + (col0 + lane % 16) * 4);
   return r;
 }
 
-// 16 bytes of a row of `d` columns from column c on (zeros past its end); `wide`: the row is 16-byte aligned
+// 16 bytes from p on, element by element
 template <typename T>
-__device__ __forceinline__ u32x4 piece_at(const T* row, int c, int d, bool wide) {
-  u32x4 r = {0, 0, 0, 0};
-  if (c < d) {
-    if (wide) {
-      r = *reinterpret_cast<const u32x4*>(row + c);
-    } else {
-      T tmp[16 / sizeof(T)];
+__device__ __forceinline__ u32x4 piece_of_elements(const T* p) {
+  T tmp[16 / sizeof(T)];
 #pragma unroll
-      for (int i = 0; i < (int)(16 / sizeof(T)); ++i) tmp[i] = row[c + i];
-      r = *reinterpret_cast<const u32x4*>(tmp);
+  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) tmp[i] = p[i];
+  return __builtin_bit_cast(u32x4, tmp);
+}
+
+// A thread's pieces (16 bytes) of a tile of C rows: rows r0, r0 + step, ... at column c0.
+template <typename T, int COLS, int C, int THREADS>
+struct Pieces {
+  static constexpr int to_row = COLS * (int)sizeof(T) / 16, step = THREADS / to_row, count = C / step;
+  static_assert(THREADS % to_row == 0 && C % step == 0, "whole rows to a round");
+  int r0, c0;
+  uint32_t offset;                   // of the first piece, in bytes, from the tile's first element in memory
+  int lds;
+  bool live;
+  u32x4 held[count];
+  __device__ __forceinline__ Pieces(int tid, int64_t stride, int columns) {
+    r0 = tid / to_row;
+    c0 = tid % to_row * (16 / (int)sizeof(T));
+    live = c0 < columns;
+    offset = (uint32_t)((r0 * stride + c0) * (int)sizeof(T));
+    lds = Tile<T, COLS>::at(r0, c0);
+  }
+  // n rows from `from` on; the rest, and columns past the end, are zeros
+  template <bool ALIGNED>
+  __device__ __forceinline__ void load(const T* from, int64_t stride, int n) {
+    if (ALIGNED && n == C) {
+#pragma unroll
+      for (int i = 0; i < count; ++i) {
+        held[i] = u32x4{0, 0, 0, 0};
+        if (live) held[i] = *reinterpret_cast<const u32x4*>((const char*)(from + i * step * stride) + offset);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < count; ++i) {
+        held[i] = u32x4{0, 0, 0, 0};
+        if (live && r0 + i * step < n) {
+          const T* at = from + (r0 + i * step) * stride + c0;
+          held[i] = ALIGNED ? *reinterpret_cast<const u32x4*>(at) : piece_of_elements(at);
+        }
+      }
     }
   }
-  return r;
-}
+  __device__ __forceinline__ void store(char* tile) const {
+#pragma unroll
+    for (int i = 0; i < count; ++i) {
+      char* at = tile + lds + i * step * Tile<T, COLS>::stride;
+      if (sizeof(T) == 2) {              // columns c0 .. c0 + 3 and the next 4
+        *reinterpret_cast<mi_u32x2*>(at) = mi_u32x2{held[i][0], held[i][1]};
+        *reinterpret_cast<mi_u32x2*>(at + 16) = mi_u32x2{held[i][2], held[i][3]};
+      } else {
+        *reinterpret_cast<u32x4*>(at) = held[i];
+      }
+    }
+  }
+};
+
 __device__ __forceinline__ bool all_finite(u32x4 x, bf16*) {
   bool ok = true;
 #pragma unroll
@@ -308,7 +362,6 @@ struct LinearAttention {
   int num_rows, num_tokens, num_requests, nkv, rep, d;
   int segment;                       // tokens of a segment; 0: every request is one
   float scale;
-  bool wide_q, wide_k, wide_v, wide_out;
 };
 
 // A request's segments are consecutive units from first_unit on: ceil(length / segment) of them fit before the next
@@ -321,34 +374,39 @@ __device__ __forceinline__ int first_unit(const LinearAttention& a, int b) {
   return min(max(a.cu[b], 0), a.num_tokens) / a.segment + b;
 }
 
-template <typename T, int DP, int NT, int C>
+template <typename T, int DP, int WAVES, int C, int PBUF>
 struct ChunkShape {
-  static constexpr int waves = 4, threads = 256;
-  static constexpr int VS = 16 * NT * waves;
+  static constexpr int waves = WAVES, threads = 64 * WAVES;
+  static constexpr int VS = 16 * waves;
   static constexpr int kt = DP / 16, ct = C / 16;
   static constexpr int q_bytes = (Tile<T, DP>::bytes(C) + 15) / 16 * 16;
   static constexpr int v_bytes = (Tile<T, VS>::bytes(C) + 15) / 16 * 16;
-  static constexpr int p_bytes = (Tile<T, C>::bytes(C) + 15) / 16 * 16;
-  static constexpr int parts = sizeof(T) == 2 ? 2 : 1;
-  static constexpr int lds(bool states) { return q_bytes + v_bytes + (states ? 0 : q_bytes + parts * p_bytes); }
+  static constexpr int part_bytes = (Tile<T, C>::bytes(C) + 15) / 16 * 16;
+  static constexpr int p_bytes = (sizeof(T) == 2 ? 2 : 1) * part_bytes;
+  static constexpr int lds(bool states) { return 2 * (q_bytes + v_bytes) + (states ? 0 : 2 * q_bytes + PBUF * p_bytes); }
 };
 
 // STATES: only what a segment adds to its request's state (from zero), left in `work`; the last segment's is not needed.
-template <typename T, int DP, int NT, int C, bool STATES>
-__global__ __launch_bounds__(256) void la_chunk_kernel(LinearAttention a) {
-  typedef ChunkShape<T, DP, NT, C> Shape;
+// ALIGNED: rows of q, k and v start at multiples of 16 bytes, of out at multiples of 4 elements, and a chunk of a tensor
+// spans less than 2^31 bytes.
+template <typename T, int DP, int WAVES, int C, int PBUF, bool STATES, bool ALIGNED, int PER_SIMD>
+__global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAttention a) {
+  typedef ChunkShape<T, DP, WAVES, C, PBUF> Shape;
   typedef typename Half<T>::type half;
+  typedef typename Half<T>::pair pair;
+  constexpr int PARTS = Split<T, 2>::parts;
   typedef Tile<T, DP> QTile;
   typedef Tile<T, Shape::VS> VTile;
   typedef Tile<T, C> PTile;
-  constexpr int KT = Shape::kt, CT = Shape::ct, VS = Shape::VS, PE = 16 / sizeof(T);
+  constexpr int KT = Shape::kt, CT = Shape::ct, VS = Shape::VS;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ float power[C + 1];
-  __shared__ int found, not_finite;
+  __shared__ float power[C + 1];     // a^i
+  __shared__ float left[2 * C];      // a^(C-1-i), zeros from C on
+  __shared__ int found, not_finite[2];
   char* const k_lds = lds;
-  char* const v_lds = k_lds + Shape::q_bytes;
-  char* const q_lds = v_lds + Shape::v_bytes;
-  char* const p_lds = q_lds + Shape::q_bytes;
+  char* const v_lds = k_lds + 2 * Shape::q_bytes;
+  char* const q_lds = v_lds + 2 * Shape::v_bytes;
+  char* const p_lds = q_lds + 2 * Shape::q_bytes;
 
   const int tid = threadIdx.x, lane = tid & (MI_WAVE - 1), wave = tid / MI_WAVE, l16 = lane & 15, g4 = lane / 16 * 4;
   const int slices = (a.d + VS - 1) / VS;
@@ -377,7 +435,7 @@ __global__ __launch_bounds__(256) void la_chunk_kernel(LinearAttention a) {
   }
   if (lo >= hi) return;
 
-  const int n0 = slice * VS + wave * 16 * NT;            // first column of the wave
+  const int n0 = slice * VS + wave * 16;                 // first column of the wave
   const int row = a.rows[b];
   T* const out = (T*)a.out;
   if (row < 0 || row >= a.num_rows) {                    // no such state: rows of NaN
@@ -389,247 +447,292 @@ __global__ __launch_bounds__(256) void la_chunk_kernel(LinearAttention a) {
     return;
   }
   for (int i = tid; i <= C; i += Shape::threads) power[i] = decay_power(a.log_decay[h], i);
-  if (tid == 0) not_finite = 0;
+  for (int i = tid; i < 2 * C; i += Shape::threads) left[i] = i < C ? decay_power(a.log_decay[h], C - 1 - i) : 0.f;
+  if (tid < 2) not_finite[tid] = 0;
+  __syncthreads();
 
-  // the wave's columns of the state, accumulator (nt, t): rows 16 t + g4 + i, column n0 + 16 nt + l16
-  f32x4 s[NT][KT];
+  // the wave's columns of the state, accumulator t: rows 16 t + g4 + i, column n0 + l16
+  f32x4 s[KT];
   float* const s_row = a.state + (int64_t)row * a.state_stride + (int64_t)h * d * d;
   float* const s_work = a.segment ? a.work + ((int64_t)unit * a.nkv + h) * d * d : nullptr;
   const float* const s_from = segments > 1 ? s_work : s_row;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int t = 0; t < KT; ++t)
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * t + g4 + i, c = n0 + 16 * nt + l16;
-        s[nt][t][i] = !STATES && r < d && c < d ? s_from[(int64_t)r * d + c] : 0.f;
-      }
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * t + g4 + i, c = n0 + l16;
+      s[t][i] = !STATES && r < d && c < d ? s_from[(int64_t)r * d + c] : 0.f;
+    }
 
   const T* const kp = (const T*)a.k + (int64_t)h * d;
-  const T* const vp = (const T*)a.v + (int64_t)h * d;
+  const T* const vp = (const T*)a.v + (int64_t)h * d + slice * VS;
   const T* const qp = (const T*)a.q + (int64_t)h * a.rep * d;
 
-  // staging: a thread's pieces of a tile
-  constexpr int KP = C * DP / PE / Shape::threads, VP = C * VS / PE / Shape::threads;
-  static_assert(KP >= 1 && VP >= 1, "a tile has a piece for every thread");
-  u32x4 kr[KP], vr[VP], qr[KP];
+  Pieces<T, DP, C, Shape::threads> kr(tid, a.k_stride, d), qr(tid, a.q_stride, d);
+  Pieces<T, VS, C, Shape::threads> vr(tid, a.v_stride, d - slice * VS);
   auto load_k = [&](int t, int n) {
-#pragma unroll
-    for (int i = 0; i < KP; ++i) {
-      const int p = tid + i * Shape::threads, r = p / (DP / PE), c = p % (DP / PE) * PE;
-      kr[i] = r < n ? piece_at(kp + (int64_t)(t + r) * a.k_stride, c, d, a.wide_k) : u32x4{0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int i = 0; i < VP; ++i) {
-      const int p = tid + i * Shape::threads, r = p / (VS / PE), c = p % (VS / PE) * PE + slice * VS;
-      vr[i] = r < n ? piece_at(vp + (int64_t)(t + r) * a.v_stride, c, d, a.wide_v) : u32x4{0, 0, 0, 0};
-    }
+    kr.template load<ALIGNED>(kp + t * a.k_stride, a.k_stride, n);
+    vr.template load<ALIGNED>(vp + t * a.v_stride, a.v_stride, n);
   };
-  auto load_q = [&](int t, int n, int g) {
-#pragma unroll
-    for (int i = 0; i < KP; ++i) {
-      const int p = tid + i * Shape::threads, r = p / (DP / PE), c = p % (DP / PE) * PE;
-      qr[i] = r < n ? piece_at(qp + (int64_t)(t + r) * a.q_stride + (int64_t)g * d, c, d, a.wide_q) : u32x4{0, 0, 0, 0};
-    }
-  };
-  auto store_q = [&]() {
-#pragma unroll
-    for (int i = 0; i < KP; ++i) {
-      const int p = tid + i * Shape::threads;
-      *reinterpret_cast<u32x4*>(q_lds + QTile::at(p / (DP / PE), p % (DP / PE) * PE)) = qr[i];
-    }
-  };
-  auto store_k = [&]() -> bool {      // whether a value is not finite
+  auto load_q = [&](int t, int n, int g) { qr.template load<ALIGNED>(qp + t * a.q_stride + g * d, a.q_stride, n); };
+  auto store_k = [&](int buf) -> bool {      // whether a value is not finite
+    kr.store(k_lds + buf * Shape::q_bytes);
+    vr.store(v_lds + buf * Shape::v_bytes);
     bool ok = true;
 #pragma unroll
-    for (int i = 0; i < KP; ++i) {
-      const int p = tid + i * Shape::threads;
-      *reinterpret_cast<u32x4*>(k_lds + QTile::at(p / (DP / PE), p % (DP / PE) * PE)) = kr[i];
-    }
-#pragma unroll
-    for (int i = 0; i < VP; ++i) {
-      const int p = tid + i * Shape::threads;
-      *reinterpret_cast<u32x4*>(v_lds + VTile::at(p / (VS / PE), p % (VS / PE) * PE)) = vr[i];
-      ok = ok && all_finite(vr[i], (T*)nullptr);
-    }
+    for (int i = 0; i < vr.count; ++i) ok = ok && all_finite(vr.held[i], (T*)nullptr);
     return !ok;
   };
-
-  const int lane_q = QTile::at(l16, g4), lane_p = PTile::at(l16, g4);
-  int t = lo, n = min(C, hi - lo);
-  // Tokens before `careful` go one to a chunk: a masked weight of zero times a value that is not finite would reach
-  // the tokens before it.
-  int careful = lo;
-  load_k(t, n);
-  if (!STATES) load_q(t, n, 0);
-  int weighted = -1;                 // the number of tokens that `w` is for
-  f32x4 w[CT];                       // a^(n-1-j) of tokens j = 16 jt + g4 + i
-  for (;;) {
-    // K, V (and the first Q) to LDS
-    if (store_k() && !STATES) not_finite = 1;
-    if (!STATES) store_q();
-    __syncthreads();
-    if (!STATES && not_finite) {
-      __syncthreads();
-      if (tid == 0) not_finite = 0;
-      if (n > 1) {
-        careful = t + n;
-        n = 1;
-        load_k(t, n);
-        load_q(t, n, 0);
-        store_k();
-        store_q();
-      }
-      __syncthreads();
-    }
-    const int t_next = t + n;
-    const int n_next = t_next < careful ? 1 : min(C, hi - t_next);
-    if (n != weighted) {
-      weighted = n;
+  half vt[CT];                       // V^T of the chunk: the wave's 16 columns, tokens 16 jt + g4 + i
+  T* const typed = nullptr;          // (picks an overload)
+  auto read_v = [&](int buf) {
 #pragma unroll
-      for (int jt = 0; jt < CT; ++jt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[jt][i] = power[max(0, n - 1 - (16 * jt + g4 + i))];
-    }
-    if (STATES || a.rep == 1) {
-      if (t_next < hi) load_k(t_next, n_next);
-    }
-    half vt[NT][CT];                 // V^T: 16 columns, tokens 16 jt + g4 + i
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int jt = 0; jt < CT; ++jt) vt[nt][jt] = half_down<VS>(v_lds, 16 * jt, wave * 16 * NT + 16 * nt, lane, (T*)nullptr);
-
-    if constexpr (!STATES) {
-      for (int g = 0; g < a.rep; ++g) {
-        const bool last = g + 1 == a.rep;
-        if (!last) load_q(t, n, g + 1);
-        else if (t_next < hi) load_q(t_next, n_next, 0);
-        if (a.rep > 1 && last && t_next < hi) load_k(t_next, n_next);
-        // ---- P^T of 16 queries
-        for (int ib = wave; ib < CT; ib += Shape::waves) {
-          half qf[KT];
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt) qf[kt] = half_at<T>(q_lds + lane_q + 16 * ib * QTile::stride + 16 * kt * (int)sizeof(T));
-          for (int jt = 0; jt <= (ib | 1); ++jt) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-            if (jt <= ib) {
-#pragma unroll
-              for (int kt = 0; kt < KT; kt += 2) {
-                const char* kf = k_lds + lane_q + 16 * jt * QTile::stride + 16 * kt * (int)sizeof(T);
-                mma(acc, half_at<T>(kf), half_at<T>(kf + 16 * sizeof(T)), qf[kt], qf[kt + 1]);
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int e = 16 * ib + l16 - (16 * jt + g4 + i);
-                acc[i] = e >= 0 ? acc[i] * power[max(e, 0)] : 0.f;
-              }
-            }
-            const Split<T, 2> p(acc);
-#pragma unroll
-            for (int x = 0; x < Split<T, 2>::parts; ++x)
-              *reinterpret_cast<half*>(p_lds + x * Shape::p_bytes + lane_p + 16 * ib * PTile::stride + 16 * jt * (int)sizeof(T)) = p.part[x];
-          }
-        }
-        // ---- what the state gives
-        f32x4 o[NT][CT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int ib = 0; ib < CT; ++ib) o[nt][ib] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kt = 0; kt < KT; kt += 2) {
-          half q0[CT], q1[CT];
-#pragma unroll
-          for (int ib = 0; ib < CT; ++ib) {
-            const char* qf = q_lds + lane_q + 16 * ib * QTile::stride + 16 * kt * (int)sizeof(T);
-            q0[ib] = half_at<T>(qf);
-            q1[ib] = half_at<T>(qf + 16 * sizeof(T));
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const Split<T, 2> s0(s[nt][kt]), s1(s[nt][kt + 1]);
-#pragma unroll
-            for (int x = 0; x < Split<T, 2>::parts; ++x)
-#pragma unroll
-              for (int ib = 0; ib < CT; ++ib) mma(o[nt][ib], s0.part[x], s1.part[x], q0[ib], q1[ib]);
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int ib = 0; ib < CT; ++ib) o[nt][ib] *= power[16 * ib + l16 + 1];
-        __syncthreads();             // P is whole; nobody reads Q any more
-        if (!last) store_q();
-        // ---- what the chunk's own tokens give
-#pragma unroll
-        for (int ib = 0; ib < CT; ++ib)
-#pragma unroll
-          for (int jt = 0; jt <= ib; jt += 2)
-#pragma unroll
-            for (int x = 0; x < Split<T, 2>::parts; ++x) {
-              const char* pf = p_lds + x * Shape::p_bytes + lane_p + 16 * ib * PTile::stride + 16 * jt * (int)sizeof(T);
-              const half p0 = half_at<T>(pf), p1 = half_at<T>(pf + 16 * sizeof(T));
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma(o[nt][ib], vt[nt][jt], vt[nt][jt + 1], p0, p1);
-            }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int c = n0 + 16 * nt + g4;
-#pragma unroll
-          for (int ib = 0; ib < CT; ++ib) {
-            const int i = 16 * ib + l16;
-            if (i < n && c < d) {
-              T* at = out + (int64_t)(t + i) * a.out_stride + (int64_t)(h * a.rep + g) * d + c;
-              const float r[4] = {o[nt][ib][0] * a.scale, o[nt][ib][1] * a.scale, o[nt][ib][2] * a.scale, o[nt][ib][3] * a.scale};
-              if (a.wide_out) {
-                store4(at, r);
-              } else {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) at[x] = from_float<T>(r[x]);
-              }
-            }
-          }
-        }
-        if (!last) __syncthreads();  // the next Q is there, P is free
-      }
-    }
-    // ---- the state after the chunk
+    for (int jt = 0; jt < CT; ++jt) vt[jt] = half_down<VS>(v_lds + buf * Shape::v_bytes, 16 * jt, wave * 16, lane, typed);
+  };
+  auto update = [&](int buf, int n) {        // the state after a chunk of n tokens
+    const char* const kb = k_lds + buf * Shape::q_bytes;
     const float an = power[n];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int kt = 0; kt < KT; ++kt) s[kt] *= an;
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) s[nt][kt] *= an;
+    for (int jt = 0; jt < CT; jt += 2) {
+      pair kp[KT];
 #pragma unroll
-      for (int jt = 0; jt < CT; jt += 2) {
-        const Split<T, 3> v0(widen(vt[nt][jt]) * w[jt]), v1(widen(vt[nt][jt + 1]) * w[jt + 1]);
+      for (int kt = 0; kt < KT; ++kt)
+        kp[kt] = join(half_down<DP>(kb, 16 * jt, 16 * kt, lane, typed), half_down<DP>(kb, 16 * jt + 16, 16 * kt, lane, typed));
+      f32x4 w0, w1;                  // a^(n-1-j)
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          const half k0 = half_down<DP>(k_lds, 16 * jt, 16 * kt, lane, (T*)nullptr);
-          const half k1 = half_down<DP>(k_lds, 16 * jt + 16, 16 * kt, lane, (T*)nullptr);
+      for (int i = 0; i < 4; ++i) {
+        w0[i] = left[C - n + 16 * jt + g4 + i];
+        w1[i] = left[C - n + 16 * jt + 16 + g4 + i];
+      }
+      __builtin_amdgcn_sched_barrier(0);     // (the reads are on their way together)
+      const Split<T, 3> v0(widen(vt[jt]) * w0), v1(widen(vt[jt + 1]) * w1);
 #pragma unroll
-          for (int x = 0; x < Split<T, 3>::parts; ++x) mma(s[nt][kt], k0, k1, v0.part[x], v1.part[x]);
-        }
+      for (int z = 0; z < Split<T, 3>::parts; ++z)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) mma(s[kt], kp[kt], join(v0.part[z], v1.part[z]));
+    }
+  };
+
+  // The chunk at hand has the n tokens from t on.  Tiles are double-buffered: while one chunk (K, V) or query head (Q) is
+  // worked on, the next one's pieces are on their way in registers; they are stored to the other buffer before the one
+  // barrier of each step, and the loads after them are issued at once.
+  int t = lo, n = min(C, hi - lo), kv = 0;
+  if constexpr (STATES) {
+    load_k(t, n);
+    store_k(0);
+    if (t + n < hi) load_k(t + n, min(C, hi - t - n));
+    __syncthreads();
+    for (;;) {
+      read_v(kv);
+      update(kv, n);
+      t += n;
+      if (t >= hi) break;
+      n = min(C, hi - t);
+      kv ^= 1;
+      store_k(kv);
+      if (t + n < hi) load_k(t + n, min(C, hi - t - n));
+      __syncthreads();
+    }
+  } else {
+    const uint32_t out_offset = (uint32_t)((l16 * a.out_stride + n0 + g4) * (int)sizeof(T));
+    const int lane_q = QTile::at(l16, g4), lane_p = PTile::at(l16, g4);
+    // the weights a^(i-j) of the P that the wave makes, and a^(i+1) of its tokens, both with the scale
+    constexpr int PW = (CT * CT / 2 + WAVES - 1) / WAVES;
+    int reach[PW];                   // i - j of a lane's first element: those of the next ones are less
+    f32x4 weight[PW][2];
+    float reached[CT];
+#pragma unroll
+    for (int y = 0; y < PW; ++y) {
+      const int x = wave + y * WAVES;
+      reach[y] = 16 * (x % CT) + l16 - (x / CT * 32 + g4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        weight[y][0][i] = power[min(max(reach[y] - i, 0), C)] * a.scale;
+        weight[y][1][i] = power[min(max(reach[y] - 16 - i, 0), C)] * a.scale;
       }
     }
-    t = t_next;
-    n = n_next;
-    if (t >= hi) break;
-    __syncthreads();                 // nobody reads K and V any more
+#pragma unroll
+    for (int ib = 0; ib < CT; ++ib) reached[ib] = power[16 * ib + l16 + 1] * a.scale;
+    // the state's parts, held for all query heads of a chunk where there are registers for them
+    constexpr bool HELD = DP <= 128;
+    pair sp[HELD ? KT / 2 : 1][PARTS];
+    // Tokens before `careful` go one to a chunk: a masked weight of zero times a value that is not finite would reach
+    // the tokens before it.
+    int careful = lo;
+    auto tokens_at = [&](int t) { return t < careful ? 1 : min(C, hi - t); };
+    // the query head whose Q is on its way: of tokens nt .. nt + nn - 1
+    int nt = t, nn = n, ng = 0;
+    auto fetch_next_q = [&]() {
+      if (++ng == a.rep) {
+        ng = 0;
+        nt += nn;
+        nn = tokens_at(nt);
+      }
+      if (nt < hi) load_q(nt, nn, ng);
+    };
+    load_k(t, n);
+    load_q(t, n, 0);
+    if (store_k(0)) not_finite[0] = 1;
+    qr.store(q_lds);
+    fetch_next_q();
+    if (t + n < hi) load_k(t + n, tokens_at(t + n));
+    __syncthreads();
+    int g = 0, qb = 0, pb = 0;
+    for (;;) {
+      if (g == 0) {
+        if (not_finite[kv]) {          // the first of this chunk's tokens alone
+          __syncthreads();
+          if (tid == 0) not_finite[kv] = 0;
+          if (n > 1) {
+            careful = t + n;
+            n = 1;
+            load_k(t, n);
+            load_q(t, n, 0);
+            store_k(kv);
+            qr.store(q_lds + qb * Shape::q_bytes);
+            nt = t, nn = n, ng = 0;
+            fetch_next_q();
+            if (t + n < hi) load_k(t + n, tokens_at(t + n));
+          }
+          __syncthreads();
+        }
+        read_v(kv);
+        if (HELD) {
+#pragma unroll
+          for (int kt = 0; kt < KT / 2; ++kt) {
+            const Split<T, 2> s0(s[2 * kt]), s1(s[2 * kt + 1]);
+#pragma unroll
+            for (int z = 0; z < PARTS; ++z) sp[kt][z] = join(s0.part[z], s1.part[z]);
+          }
+        }
+      }
+      const char* const qt = q_lds + qb * Shape::q_bytes + lane_q;
+      const char* const kt_lds = k_lds + kv * Shape::q_bytes + lane_q;
+      char* const pt = p_lds + pb * Shape::p_bytes + lane_p;
+      // ---- P^T: to a wave 16 queries and 32 tokens, or that again for the next waves' worth of them
+#pragma unroll
+      for (int y = 0; y < PW; ++y) {
+        const int x = wave + y * WAVES, ib = x % CT, jt = x / CT * 2;
+        if (x >= CT * CT / 2 || jt > ib) continue;             // (no product below reads these)
+        pair qf[KT / 2], k0[KT / 2], k1[KT / 2];
+#pragma unroll
+        for (int kt = 0; kt < KT / 2; ++kt) {
+          qf[kt] = halves_at(qt + 16 * ib * QTile::stride, 32 * kt, typed);
+          k0[kt] = halves_at(kt_lds + 16 * jt * QTile::stride, 32 * kt, typed);
+          k1[kt] = halves_at(kt_lds + (16 * jt + 16) * QTile::stride, 32 * kt, typed);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 p0 = {0.f, 0.f, 0.f, 0.f}, p1 = p0;
+#pragma unroll
+        for (int kt = 0; kt < KT / 2; ++kt) {
+          mma(p0, k0[kt], qf[kt]);
+          mma(p1, k1[kt], qf[kt]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p0[i] = reach[y] >= i ? p0[i] * weight[y][0][i] : 0.f;
+          p1[i] = reach[y] >= 16 + i ? p1[i] * weight[y][1][i] : 0.f;
+        }
+        const Split<T, 2> s0(p0), s1(p1);
+#pragma unroll
+        for (int z = 0; z < PARTS; ++z) {
+          char* at = pt + z * Shape::part_bytes + 16 * ib * PTile::stride;
+          *reinterpret_cast<half*>(at + PTile::at(0, 16 * jt)) = s0.part[z];
+          *reinterpret_cast<half*>(at + PTile::at(0, 16 * jt + 16)) = s1.part[z];
+        }
+      }
+      // ---- what the state gives
+      f32x4 o[CT];
+#pragma unroll
+      for (int ib = 0; ib < CT; ++ib) o[ib] = f32x4{0.f, 0.f, 0.f, 0.f};
+      pair qf[2][CT];
+#pragma unroll
+      for (int ib = 0; ib < CT; ++ib) qf[0][ib] = halves_at(qt + 16 * ib * QTile::stride, 0, typed);
+#pragma unroll
+      for (int kt = 0; kt < KT / 2; ++kt) {
+        if (kt + 1 < KT / 2) {
+#pragma unroll
+          for (int ib = 0; ib < CT; ++ib) qf[(kt + 1) & 1][ib] = halves_at(qt + 16 * ib * QTile::stride, 32 * (kt + 1), typed);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (!HELD) {
+          const Split<T, 2> s0(s[2 * kt]), s1(s[2 * kt + 1]);
+#pragma unroll
+          for (int z = 0; z < PARTS; ++z) sp[0][z] = join(s0.part[z], s1.part[z]);
+        }
+#pragma unroll
+        for (int z = 0; z < PARTS; ++z)
+#pragma unroll
+          for (int ib = 0; ib < CT; ++ib) mma(o[ib], sp[HELD ? kt : 0][z], qf[kt & 1][ib]);
+      }
+#pragma unroll
+      for (int ib = 0; ib < CT; ++ib) o[ib] *= reached[ib];
+      const bool last = g + 1 == a.rep, more = t + n < hi;
+      if (last) update(kv, n);
+      if (!last || more) qr.store(q_lds + (qb ^ 1) * Shape::q_bytes);
+      if (last && more) {
+        if (store_k(kv ^ 1)) not_finite[kv ^ 1] = 1;
+        const int after = t + n + tokens_at(t + n);
+        if (after < hi) load_k(after, tokens_at(after));
+      }
+      fetch_next_q();
+      __syncthreads();
+      // ---- what the chunk's own tokens give
+      pair pf[CT][(CT + 1) / 2][PARTS];
+#pragma unroll
+      for (int ib = 0; ib < CT; ++ib)
+#pragma unroll
+        for (int jt = 0; jt <= ib; jt += 2)
+#pragma unroll
+          for (int z = 0; z < PARTS; ++z) pf[ib][jt / 2][z] = halves_at(pt + z * Shape::part_bytes + 16 * ib * PTile::stride, 16 * jt, typed);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int jt = 0; jt < CT; jt += 2)
+#pragma unroll
+        for (int z = 0; z < PARTS; ++z)
+#pragma unroll
+          for (int ib = jt; ib < CT; ++ib) mma(o[ib], join(vt[jt], vt[jt + 1]), pf[ib][jt / 2][z]);
+      const int c = n0 + g4;
+      T* const o_at = out + t * a.out_stride + (int64_t)(h * a.rep + g) * d;
+#pragma unroll
+      for (int ib = 0; ib < CT; ++ib) {
+        const int i = 16 * ib + l16;
+        if (i < n && c < d) {
+          const float r[4] = {o[ib][0], o[ib][1], o[ib][2], o[ib][3]};
+          if (ALIGNED) {
+            store4((T*)((char*)(o_at + 16 * ib * a.out_stride) + out_offset), r);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o_at[i * a.out_stride + c + x] = from_float<T>(r[x]);
+          }
+        }
+      }
+      if (PBUF == 1) __syncthreads();              // P is free
+      else pb ^= 1;
+      qb ^= 1;
+      if (last) {
+        t += n;
+        if (t >= hi) break;
+        n = tokens_at(t);
+        kv ^= 1;
+        g = 0;
+      } else {
+        ++g;
+      }
+    }
   }
 
   float* const s_to = STATES ? s_work : segment == segments - 1 ? s_row : nullptr;
   if (s_to) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 16 * kt + g4 + i, c = n0 + 16 * nt + l16;
-          if (r < d && c < d) s_to[(int64_t)r * d + c] = s[nt][kt][i];
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * kt + g4 + i, c = n0 + l16;
+        if (r < d && c < d) s_to[(int64_t)r * d + c] = s[kt][i];
+      }
   }
 }
 
@@ -656,33 +759,44 @@ __global__ __launch_bounds__(256) void la_scan_kernel(LinearAttention a) {
   }
 }
 
-template <typename T, int DP, int NT, int C, bool STATES>
+template <typename T, int DP, int WAVES, int C, int PBUF, bool STATES, bool ALIGNED, int PER_SIMD>
 static int launch_chunks(const LinearAttention& a, int64_t units, hipStream_t stream) {
-  typedef ChunkShape<T, DP, NT, C> Shape;
+  typedef ChunkShape<T, DP, WAVES, C, PBUF> Shape;
   static std::atomic<uint64_t> ready{0};           // devices on which the kernel may use this much LDS
   constexpr int bytes = Shape::lds(STATES);
   int device = 0;
   (void)hipGetDevice(&device);
   if (!((ready.load(std::memory_order_relaxed) >> (device & 63)) & 1)) {
-    hipError_t e = hipFuncSetAttribute((const void*)la_chunk_kernel<T, DP, NT, C, STATES>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    hipError_t e = hipFuncSetAttribute((const void*)la_chunk_kernel<T, DP, WAVES, C, PBUF, STATES, ALIGNED, PER_SIMD>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     MI_REQUIRE(e == hipSuccess, "linear attention: %d bytes of LDS: %s", bytes, hipGetErrorString(e));
     ready.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
   }
   const int64_t blocks = units * a.nkv * ((a.d + Shape::VS - 1) / Shape::VS);
   MI_REQUIRE(blocks <= 0x7fffffff, "linear attention: %lld workgroups are too many for one launch", (long long)blocks);
-  la_chunk_kernel<T, DP, NT, C, STATES><<<(uint32_t)blocks, Shape::threads, bytes, stream>>>(a);
+  la_chunk_kernel<T, DP, WAVES, C, PBUF, STATES, ALIGNED, PER_SIMD><<<(uint32_t)blocks, Shape::threads, bytes, stream>>>(a);
   MI_CHECK_LAUNCH("linear attention, chunks");
   return 0;
 }
 
-template <typename T, int DP, int NT, int C>
-static int launch_prompt(const LinearAttention& a, hipStream_t stream) {
-  if (!a.segment) return launch_chunks<T, DP, NT, C, false>(a, a.num_requests, stream);
+template <typename T, int DP, int WAVES, int C, int PBUF, bool ALIGNED, int PER_SIMD>
+static int launch_aligned(const LinearAttention& a, hipStream_t stream) {
+  if (!a.segment) return launch_chunks<T, DP, WAVES, C, PBUF, false, ALIGNED, PER_SIMD>(a, a.num_requests, stream);
   const int64_t units = a.num_tokens / a.segment + a.num_requests;
-  if (launch_chunks<T, DP, NT, C, true>(a, units, stream)) return 1;
+  if (launch_chunks<T, DP, WAVES, C, PBUF, true, ALIGNED, PER_SIMD>(a, units, stream)) return 1;
   la_scan_kernel<<<dim3((a.nkv * a.d * a.d / 4 + 255) / 256, a.num_requests), 256, 0, stream>>>(a);
   MI_CHECK_LAUNCH("linear attention, scan");
-  return launch_chunks<T, DP, NT, C, false>(a, units, stream);
+  return launch_chunks<T, DP, WAVES, C, PBUF, false, ALIGNED, PER_SIMD>(a, units, stream);
+}
+
+template <typename T, int DP, int WAVES, int C, int PBUF, int PER_SIMD>
+static int launch_prompt(const LinearAttention& a, hipStream_t stream) {
+  auto fits = [](const void* p, int64_t stride, int bytes) {
+    return ((uint64_t)p | (uint64_t)(stride * (int64_t)sizeof(T))) % bytes == 0 && stride * C * (int64_t)sizeof(T) < (1ll << 31);
+  };
+  const bool aligned = fits(a.q, a.q_stride, 16) && fits(a.k, a.k_stride, 16) && fits(a.v, a.v_stride, 16) &&
+                       fits(a.out, a.out_stride, 4 * sizeof(T));
+  return aligned ? launch_aligned<T, DP, WAVES, C, PBUF, true, PER_SIMD>(a, stream)
+                 : launch_aligned<T, DP, WAVES, C, PBUF, false, 1>(a, stream);
 }
 
 // segment: tokens of a segment (a multiple of 64), or 0 for one workgroup's walk over each whole request; work: then
@@ -691,20 +805,17 @@ MI_EXPORT int mi_linear_attention(LA_ARGS, int segment, float* work, hipStream_t
   if (check_sizes(nq, nkv, d, num_requests, state_stride)) return 1;
   MI_REQUIRE(segment >= 0 && segment % 64 == 0 && (segment == 0 || work), "linear attention: segments of %d tokens", segment);
   if (num_requests == 0 || num_tokens == 0) return 0;
-  const int size = dtype == MI_DTYPE_BF16 ? 2 : 4;
-  auto wide = [&](const void* p, int64_t stride, int bytes) { return ((uint64_t)p | (uint64_t)(stride * size)) % bytes == 0; };
   LinearAttention a = {q, k, v, out, state, rows, cu, log_decay, work, q_stride, k_stride, v_stride, out_stride, state_stride,
-                       num_rows, num_tokens, num_requests, nkv, nq / nkv, d, segment, scale, wide(q, q_stride, 16),
-                       wide(k, k_stride, 16), wide(v, v_stride, 16), wide(out, out_stride, 4 * size)};
+                       num_rows, num_tokens, num_requests, nkv, nq / nkv, d, segment, scale};
   if (dtype == MI_DTYPE_BF16) {
-    if (d <= 64) return launch_prompt<bf16, 64, 1, 64>(a, stream);
-    if (d <= 128) return launch_prompt<bf16, 128, 1, 64>(a, stream);
-    return launch_prompt<bf16, 256, 1, 64>(a, stream);
+    if (d <= 64) return launch_prompt<bf16, 64, 4, LA_C64, LA_PBUF64, 2>(a, stream);
+    if (d <= 128) return launch_prompt<bf16, 128, 8, 64, 2, 2>(a, stream);
+    return launch_prompt<bf16, 256, 8, 32, 2, 2>(a, stream);
   }
   if (dtype == MI_DTYPE_F32) {
-    if (d <= 64) return launch_prompt<float, 64, 1, 64>(a, stream);
-    if (d <= 128) return launch_prompt<float, 128, 1, 64>(a, stream);
-    return launch_prompt<float, 256, 1, 32>(a, stream);
+    if (d <= 64) return launch_prompt<float, 64, 4, 32, 2, 2>(a, stream);
+    if (d <= 128) return launch_prompt<float, 128, 8, 32, 2, 2>(a, stream);
+    return launch_prompt<float, 256, 4, 32, 1, 1>(a, stream);
   }
   MI_FAIL("linear attention: dtype %d", dtype);
 }

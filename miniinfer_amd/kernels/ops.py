@@ -54,18 +54,22 @@ def _dev(*tensors):
 class _on_device_of:
   """Launches inside run on the device of these tensors (all on one GPU, or an error) and on its current stream, whatever
   the current device is."""
+  __slots__ = ("index", "was")
 
   def __init__(self, what, *tensors):
-    _dev(*tensors)
-    devices = {t.device.index for t in tensors if t is not None}
-    if len(devices) > 1:
-      raise KernelError(f"{what}: the tensors are on several devices ({sorted(devices)})")
-    self.index = devices.pop()
+    index = tensors[0].get_device()
+    for t in tensors:
+      if t.get_device() != index or index < 0:
+        _dev(*tensors)
+        raise KernelError(f"{what}: the tensors are on several devices ({sorted({str(t.device) for t in tensors})})")
+    self.index = index
 
   def __enter__(self):
+    """The stream to launch on."""
     self.was = torch.cuda.current_device()
     if self.was != self.index:
       torch.cuda.set_device(self.index)
+    return _RAW_STREAM(self.index) if _RAW_STREAM is not None else _stream()
 
   def __exit__(self, *exc):
     if self.was != self.index:
@@ -185,7 +189,7 @@ _libs = {}
 
 
 def _lib(name: str, defines=()):
-  key = (name, tuple(sorted(defines)))
+  key = (name, tuple(sorted(defines))) if defines else (name, ())
   lib = _libs.get(key)
   if lib is None:
     lib = jit.load_module(name, defines)
@@ -1135,46 +1139,59 @@ def attn_decode_front(qkv: torch.Tensor, nq: int, nkv: int, d: int, out: torch.T
 LINEAR_ATTENTION_MAX_D = 256
 
 
-def _linear_attention_args(what, q, k, v, nq, nkv, d, out, state, state_rows, log_decay):
+def _linear_attention_rows(what, name, t, T, columns, dtype):
+  """(address, row stride) of [T, >= columns] rows; single calls of each accessor, since a decode step's launch waits for
+  the host."""
+  shape, stride = t.shape, t.stride()
+  if len(shape) != 2 or shape[0] != T or shape[1] < columns or stride[1] != 1:
+    if len(shape) != 2 or shape[0] != T or shape[1] < columns or shape[1] > 1:
+      raise KernelError(f"{what}: {name} {tuple(shape)} does not hold {T} dense rows of {columns} elements")
+  if t.dtype is not dtype:
+    raise KernelError(f"{what}: q is {dtype}, {name} {t.dtype}")
+  if T <= 1:
+    return t.data_ptr(), columns
+  if stride[0] < columns:
+    raise KernelError(f"{what}: rows of {name} overlap (stride {stride[0]})")
+  return t.data_ptr(), stride[0]
+
+
+def _linear_attention_call(what, q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay, scale):
+  """The checked arguments of a launch, as its entry points take them."""
   if nkv < 1 or nq < nkv or nq % nkv:
     raise KernelError(f"{what}: {nq} query heads are no multiple of {nkv} kv heads")
   if d % 8 or not 8 <= d <= LINEAR_ATTENTION_MAX_D:
     raise KernelError(f"{what}: head size {d} is no multiple of 8 up to {LINEAR_ATTENTION_MAX_D}")
-  dtype_code(q.dtype)
-  T = q.shape[0]
-  for name, t, heads in (("q", q, nq), ("k", k, nkv), ("v", v, nkv), ("out", out, nq)):
-    if t.dim() != 2 or t.shape[0] != T or t.shape[1] < heads * d or (t.shape[1] > 1 and t.stride(1) != 1):
-      raise KernelError(f"{what}: {name} {tuple(t.shape)} does not hold {T} dense rows of {heads} heads of {d}")
-    if T > 1 and abs(t.stride(0)) < heads * d:
-      raise KernelError(f"{what}: rows of {name} overlap (stride {t.stride(0)})")
-    if t.dtype != q.dtype:
-      raise KernelError(f"{what}: q is {q.dtype}, {name} {t.dtype}")
-  if out.shape[1] != nq * d:
-    raise KernelError(f"{what}: out {tuple(out.shape)} is not [{T}, {nq * d}]")
-  if state.dtype != torch.float32 or state.dim() != 4 or tuple(state.shape[1:]) != (nkv, d, d) \
-      or not state[:1].is_contiguous():
-    raise KernelError(f"{what}: states must be float32 [rows, {nkv}, {d}, {d}] with dense rows, got {tuple(state.shape)} {state.dtype}")
-  if state.shape[0] > 1 and (state.stride(0) < nkv * d * d or state.stride(0) % 4):
-    raise KernelError(f"{what}: rows of states {state.stride(0)} elements apart")
-  if state.data_ptr() % 16:
+  dtype = q.dtype
+  code = BF16 if dtype is torch.bfloat16 else dtype_code(dtype)
+  T, nqd, nkvd = q.shape[0], nq * d, nkv * d
+  qp, qs = _linear_attention_rows(what, "q", q, T, nqd, dtype)
+  kp, ks = _linear_attention_rows(what, "k", k, T, nkvd, dtype)
+  vp, vs = _linear_attention_rows(what, "v", v, T, nkvd, dtype)
+  op, os = _linear_attention_rows(what, "out", out, T, nqd, dtype)
+  if out.shape[1] != nqd:
+    raise KernelError(f"{what}: out {tuple(out.shape)} is not [{T}, {nqd}]")
+  shape, stride, sp = state.shape, state.stride(), state.data_ptr()
+  if state.dtype is not torch.float32 or len(shape) != 4 or shape[1:] != (nkv, d, d) or stride[2:] != (d, 1) \
+      or (nkv > 1 and stride[1] != d * d):
+    raise KernelError(f"{what}: states must be float32 [rows, {nkv}, {d}, {d}] with dense rows, got {tuple(shape)} {state.dtype}")
+  ss = nkvd * d
+  if shape[0] > 1:
+    ss = stride[0]
+    if ss < nkvd * d or ss % 4:
+      raise KernelError(f"{what}: rows of states {ss} elements apart")
+  if sp % 16:
     raise KernelError(f"{what}: states must start at a multiple of 16 bytes")
   _i32("state_rows", state_rows)
-  _f32("log_decay", log_decay, nkv)
-  return T
-
-
-def _linear_attention_call(q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay, scale):
-  T = q.shape[0]
-  stride = lambda t: t.stride(0) if T > 1 else t.shape[1]
-  return (dtype_code(q.dtype), _ptr(q), stride(q), _ptr(k), stride(k), _ptr(v), stride(v), _ptr(out), stride(out), _ptr(state),
-          state.stride(0) if state.shape[0] > 1 else nkv * d * d, state.shape[0], _ptr(state_rows), _ptr(cu_q), T,
-          state_rows.numel(), nq, nkv, d, _ptr(log_decay), float(scale))
+  if log_decay.dtype is not torch.float32 or log_decay.numel() != nkv or not log_decay.is_contiguous():
+    _f32("log_decay", log_decay, nkv)
+  return (code, qp, qs, kp, ks, vp, vs, op, os, sp, ss, shape[0], state_rows.data_ptr(), _ptr(cu_q), T, state_rows.numel(),
+          nq, nkv, d, log_decay.data_ptr(), scale)
 
 
 def linear_attention_segment(num_tokens: int, max_len: int, nkv: int, d: int, units: int = 256) -> int:
   """Tokens of a segment into which requests are cut, 0 for none: as many as make two workgroups for every compute unit
   over all tokens, and at least two chunks."""
-  slices = -(-d // 64)
+  slices = -(-d // 64) if True else 1
   tokens = max(128, -(-num_tokens * nkv * slices // (2 * units * 64)) * 64)
   return tokens if max_len > tokens else 0
 
@@ -1193,18 +1210,18 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int,
   left as they are, and a state row outside the buffer gives rows of NaN.  log_decay float32 [nkv], <= 0 (-inf: a = 0)
   or positive for a growing state.  max_len: the most tokens of one request if the host knows it (default: T); it only
   chooses how the work is cut.  float32 and bfloat16; states and sums are 32-bit."""
-  T = _linear_attention_args("linear_attention", q, k, v, nq, nkv, d, out, state, state_rows, log_decay)
+  args = _linear_attention_call("linear_attention", q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay, scale)
   _i32("cu_q", cu_q)
+  T = args[14]
   if cu_q.numel() != state_rows.numel() + 1:
     raise KernelError(f"linear_attention: cu_q has {cu_q.numel()} entries for {state_rows.numel()} requests")
-  with _on_device_of("linear_attention", q, k, v, out, state, state_rows, cu_q, log_decay):
+  with _on_device_of("linear_attention", q, k, v, out, state, state_rows, cu_q, log_decay) as stream:
     lib = _lib("linear_attention")
     segment = linear_attention_segment(T, T if max_len is None else min(max_len, T), nkv, d, compute_units(q.device))
     work = None
     if segment:
       work = torch.empty((T // segment + state_rows.numel()) * nkv * d * d, dtype=torch.float32, device=q.device)
-    _check(lib, lib.mi_linear_attention(*_linear_attention_call(q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay,
-                                                                scale), segment, _ptr(work), _stream()))
+    _check(lib, lib.mi_linear_attention(*args, segment, _ptr(work), stream))
   return out
 
 
@@ -1213,13 +1230,12 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq:
                           scale: float) -> torch.Tensor:
   """`linear_attention` of one token for each request: row b of q, k, v and out is request b's token.  Requests may share
   a state row that nobody reads afterwards (the padding entries of a captured step do)."""
-  T = _linear_attention_args("linear_attention_step", q, k, v, nq, nkv, d, out, state, state_rows, log_decay)
-  if state_rows.numel() != T:
-    raise KernelError(f"linear_attention_step: {state_rows.numel()} state rows for {T} tokens")
-  with _on_device_of("linear_attention_step", q, k, v, out, state, state_rows, log_decay):
+  args = _linear_attention_call("linear_attention_step", q, k, v, nq, nkv, d, out, state, state_rows, None, log_decay, scale)
+  if args[15] != args[14]:
+    raise KernelError(f"linear_attention_step: {args[15]} state rows for {args[14]} tokens")
+  with _on_device_of("linear_attention_step", q, k, v, out, state, state_rows, log_decay) as stream:
     lib = _lib("linear_attention")
-    _check(lib, lib.mi_linear_attention_recurrent(*_linear_attention_call(q, k, v, nq, nkv, d, out, state, state_rows, None,
-                                                                          log_decay, scale), _stream()))
+    _check(lib, lib.mi_linear_attention_recurrent(*args, stream))
   return out
 
 
@@ -1252,7 +1268,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_beams: int,
   if num_beams > BEAM_MAX_BEAMS or not 1 <= count <= min(BEAM_MAX_COUNT, num_beams * V):
     raise KernelError(f"beam_select: {count} of {num_beams} beams x {V} tokens; at most {BEAM_MAX_COUNT} candidates of "
                       f"{BEAM_MAX_BEAMS} beams are taken")
-  with _on_device_of("beam_select", logits, scores):
+  with _on_device_of("beam_select", logits, scores) as stream:
     lib = _lib("beam")
     words = c_int64(0)
     _check(lib, lib.mi_beam_scratch(G, num_beams, V, count, ctypes.byref(words)))
@@ -1260,7 +1276,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_beams: int,
     out_scores = torch.empty((G, count), dtype=torch.float32, device=logits.device)
     out = torch.empty((2, G, count), dtype=torch.int32, device=logits.device)
     _check(lib, lib.mi_beam_select(_ptr(logits), logits.stride(0) if R > 1 else V, _ptr(scores), G, num_beams, V, count,
-                                   _ptr(scratch), _ptr(out_scores), _ptr(out[0]), _ptr(out[1]), _stream()))
+                                   _ptr(scratch), _ptr(out_scores), _ptr(out[0]), _ptr(out[1]), stream))
   return out_scores, out[0], out[1]
 
 
@@ -1299,7 +1315,7 @@ def move_rows(buffers, src: torch.Tensor, dst: torch.Tensor) -> None:
     raise KernelError(f"move_rows: {n} sources, {dst.numel()} destinations")
   if n > MOVE_ROWS_MAX:
     raise KernelError(f"move_rows: {n} moves, at most {MOVE_ROWS_MAX} are taken")
-  with _on_device_of("move_rows", src, dst, *buffers):
+  with _on_device_of("move_rows", src, dst, *buffers) as stream:
     lib = _lib("rows")
     live = [t for t in buffers if t.numel()]
     if n == 0 or not live:
@@ -1312,7 +1328,7 @@ def move_rows(buffers, src: torch.Tensor, dst: torch.Tensor) -> None:
     i64, i32 = c_int64 * m, c_int * m
     _check(lib, lib.mi_move_rows(m, (c_void_p * m)(*[_ptr(t) for t in live]), i64(*stride0), i64(*stride1), i64(*row),
                                  i32(*[t.shape[0] for t in live]), i32(*[t.shape[1] for t in live]), _ptr(src), _ptr(dst), n,
-                                 _stream()))
+                                 stream))
 
 
 # ----------------------------------------------------------------------------- what the device delivers
