@@ -177,13 +177,16 @@ _SIGS["linear_attention"] = {
 }
 
 _SIGS["beam"] = {
-  "mi_beam_select": [c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
-  "mi_beam_scratch": [c_int, c_int, c_int, c_int, c_void_p],
+  "mi_beam_select": [c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                     c_void_p],
+  "mi_beam_scratch": [c_int, c_int, c_int, c_int, c_int],
 }
 
 _SIGS["rows"] = {
   "mi_move_rows": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
 }
+
+_RESULTS = {"mi_beam_scratch": c_int64}     # entry points that return something else than an int
 
 _libs = {}
 
@@ -196,7 +199,7 @@ def _lib(name: str, defines=()):
     for fn, sig in _SIGS.get(name, {}).items():
       f = getattr(lib, fn)
       f.argtypes = sig
-      f.restype = c_int
+      f.restype = _RESULTS.get(fn, c_int)
     _libs[key] = lib
   return lib
 
@@ -1189,11 +1192,14 @@ def _linear_attention_call(what, q, k, v, nq, nkv, d, out, state, state_rows, cu
 
 
 def linear_attention_segment(num_tokens: int, max_len: int, nkv: int, d: int, units: int = 256) -> int:
-  """Tokens of a segment into which requests are cut, 0 for none: as many as make two workgroups for every compute unit
-  over all tokens, and at least two chunks."""
-  slices = -(-d // 64) if True else 1
-  tokens = max(128, -(-num_tokens * nkv * slices // (2 * units * 64)) * 64)
-  return tokens if max_len > tokens else 0
+  """Tokens of a segment into which requests are cut, 0 for none: as many (whole chunks of 64) as make one workgroup for
+  every compute unit over all tokens.  A cut costs a pass over the keys and values for the segments' states and a kernel
+  that adds them up, so a longest request of up to three segments is left whole (24 requests of up to 950 tokens, 12 heads
+  of 80: 91 us whole, 101 in segments of 448; 8 requests of 1,024 tokens, 8 heads of 128: 246 us whole, 94 in segments of
+  256)."""
+  slices = -(-d // 128)
+  tokens = max(64, -(-num_tokens * nkv * slices // (units * 64)) * 64)
+  return tokens if max_len > 3 * tokens else 0
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int, nkv: int, d: int, out: torch.Tensor,
@@ -1252,7 +1258,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_beams: int,
       scores[b] + logits[b, v] - log sum_u exp(logits[b, u])      b over the group's beams, v over the vocabulary
 
   the largest, largest first, equal ones by (beam, token).  logits float32 [G * num_beams, V] with dense rows, scores
-  float32 [G * num_beams] (-inf: a beam that does not take part).  Returns (scores float32, beams int32 in
+  float32 [G * num_beams] (-inf, or anything else that is not finite: a beam that does not take part).  Returns (scores float32, beams int32 in
   0 .. num_beams - 1, tokens int32), each [G, count].  A logit that is NaN counts as -inf; where a row holds +inf, those
   tokens share its mass; a row of -inf only has no candidate above -inf.  If fewer than `count` candidates are above -inf
   the rest of the list has score -inf.  Sums of exponentials and the scores that are compared are 64-bit."""
@@ -1265,19 +1271,20 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_beams: int,
     raise KernelError("beam_select: rows of logits overlap")
   _f32("scores", scores, R)
   G = R // num_beams
+  if num_beams * V >= 1 << 31:
+    raise KernelError(f"beam_select: {num_beams} beams x {V} tokens are too many")
   if num_beams > BEAM_MAX_BEAMS or not 1 <= count <= min(BEAM_MAX_COUNT, num_beams * V):
     raise KernelError(f"beam_select: {count} of {num_beams} beams x {V} tokens; at most {BEAM_MAX_COUNT} candidates of "
                       f"{BEAM_MAX_BEAMS} beams are taken")
   with _on_device_of("beam_select", logits, scores) as stream:
     lib = _lib("beam")
-    words = c_int64(0)
-    _check(lib, lib.mi_beam_scratch(G, num_beams, V, count, ctypes.byref(words)))
-    scratch = torch.empty(words.value, dtype=torch.float64, device=logits.device)
+    units = compute_units(logits.device)
+    scratch = torch.empty(lib.mi_beam_scratch(G, num_beams, V, count, units), dtype=torch.float64, device=logits.device)
     out_scores = torch.empty((G, count), dtype=torch.float32, device=logits.device)
-    out = torch.empty((2, G, count), dtype=torch.int32, device=logits.device)
-    _check(lib, lib.mi_beam_select(_ptr(logits), logits.stride(0) if R > 1 else V, _ptr(scores), G, num_beams, V, count,
-                                   _ptr(scratch), _ptr(out_scores), _ptr(out[0]), _ptr(out[1]), stream))
-  return out_scores, out[0], out[1]
+    beams, tokens = torch.empty((2, G, count), dtype=torch.int32, device=logits.device).unbind()
+    _check(lib, lib.mi_beam_select(logits.data_ptr(), logits.stride(0) if R > 1 else V, scores.data_ptr(), G, num_beams, V, count,
+                                   units, scratch.data_ptr(), out_scores.data_ptr(), beams.data_ptr(), tokens.data_ptr(), stream))
+  return out_scores, beams, tokens
 
 
 # ----------------------------------------------------------------------------- pages and states
