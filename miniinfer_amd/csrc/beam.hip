@@ -10,7 +10,7 @@
 //
 // Candidates of different beams lie closer to one another than a 32-bit score can tell apart (32 bits of a score of
 // -40 are steps of 4e-6, and a hundred thousand candidates share a few units), so exponentials, sums and compared scores
-// are 64-bit; the exponential is a polynomial good to 1e-11, half of the arithmetic of the pass, and hides behind the
+// are 64-bit; the exponential is a polynomial good to 3e-12, half of the arithmetic of the pass, and hides behind the
 // loads.
 #include "common.h"
 
@@ -21,52 +21,128 @@ typedef f32x4 f32x4_any __attribute__((aligned(4)));      // 16 bytes from any e
 #define BEAM_MAX_BEAMS 64
 #define BEAM_WAVES 4
 #define BEAM_THREADS (BEAM_WAVES * MI_WAVE)
+#define BEAM_FEW 1024                  // up to so many candidates of a group, four waves pick
 #define BEAM_TILE 1024                 // logits that a wave holds at once, 16 to a lane
 
 // The order of candidates.  An empty place is (-inf, INT_MAX): every real candidate comes before it.
 template <typename X>
-__device__ __forceinline__ bool before(X ax, int ai, X bx, int bi) { return ax > bx || (ax == bx && ai < bi); }
+__device__ __forceinline__ bool before(X ax, int ai, X bx, int bi) { return (ax > bx) | ((ax == bx) & (ai < bi)); }
 
 __device__ __forceinline__ float lane_value(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
 __device__ __forceinline__ double lane_value(double x, int lane) {
   return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), lane), __builtin_amdgcn_readlane(__double2loint(x), lane));
 }
-// the value one lane below (wave_shr:1); lane 0 keeps its own
-__device__ __forceinline__ int lane_below(int x) { return __builtin_amdgcn_update_dpp(x, x, 0x138, 0xf, 0xf, false); }
-__device__ __forceinline__ float lane_below(float x) { return __int_as_float(lane_below(__float_as_int(x))); }
-__device__ __forceinline__ double lane_below(double x) {
-  return __hiloint2double(lane_below(__double2hiint(x)), lane_below(__double2loint(x)));
+// The largest value of the wave, in a scalar register: four shifts within rows of 16 lanes, two broadcasts across rows.
+__device__ __forceinline__ float wave_top(float x) {
+#define STEP(CTRL, ROWS) x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), CTRL, ROWS, 0xf, false)))
+  STEP(0x111, 0xf);    // row_shr:1
+  STEP(0x112, 0xf);    // row_shr:2
+  STEP(0x114, 0xf);    // row_shr:4
+  STEP(0x118, 0xf);    // row_shr:8
+  STEP(0x142, 0xa);    // row_bcast:15 into rows 1 and 3
+  STEP(0x143, 0xc);    // row_bcast:31 into rows 2 and 3
+#undef STEP
+  return lane_value(x, 63);
 }
 
-// A wave's best candidates in order: lane l holds the l-th.
+// A wave's best candidates: lane l holds the l-th in order.  Newcomers that come before the last of the `count` that are
+// wanted gather in LDS and join 64 at a time: sorted (a bitonic network over the lanes), then merged.  One by one they
+// would cost a tenth of a microsecond each, and a wave meets `count` * (1 + ln(logits / count)) of them.
 template <typename X>
 struct Best {
   X x;
   int i;
-  int count;
-  X last_x;          // the last of the `count` that are wanted: what a newcomer has to come before
+  int count, waiting;
+  X last_x;          // the last of the `count`: what a newcomer has to come before
   int last_i;
-  __device__ __forceinline__ explicit Best(int n) : x(-INFINITY), i(INT32_MAX), count(n), last_i(INT32_MAX) {
+  X* wait_x;         // room for 63 that wait and what is taken until the next `join`
+  int* wait_i;
+  __device__ __forceinline__ Best(int n, X* wx, int* wi)
+      : x(-INFINITY), i(INT32_MAX), count(n), waiting(0), last_i(INT32_MAX), wait_x(wx), wait_i(wi) {
     // (the compiler loads a 64-bit -inf into a scalar register pair as zero, so that it must not know this value)
     asm volatile("" : "+v"(x));
     last_x = lane_value(x, 0);
   }
-  // one candidate of every lane
-  __device__ __forceinline__ void take(X nx, int ni, int lane) {
-    uint64_t mask = __ballot(before(nx, ni, last_x, last_i));
-    while (mask) {
-      const int from = __builtin_ctzll(mask);
-      const X cx = lane_value(nx, from);
-      const int ci = __builtin_amdgcn_readlane(ni, from);
-      const int place = __builtin_popcountll(__ballot(before(x, i, cx, ci)));
-      const X bx = lane_below(x);
-      const int bi = lane_below(i);
-      x = lane < place ? x : lane == place ? cx : bx;
-      i = lane < place ? i : lane == place ? ci : bi;
+  // A candidate as one number that compares as candidates do, where it fits: the float's bits made to order as whole
+  // numbers do, then the index, lower ones first.
+  static __device__ __forceinline__ uint64_t key_of(float x, int i) {
+    const uint32_t u = __float_as_uint(x + 0.f);       // (-0 and 0 are equal)
+    return (uint64_t)((u & 0x80000000u) ? ~u : (u | 0x80000000u)) << 32 | (uint32_t)~i;
+  }
+  // the wave's candidates (x, i) and those of the lanes `step` away: the better one to the lanes where `up`
+  static __device__ __forceinline__ void exchange(uint64_t& k, int step, bool up) {
+    const uint64_t o = (uint64_t)(uint32_t)__shfl_xor((int)(k >> 32), step, MI_WAVE) << 32 | (uint32_t)__shfl_xor((int)k, step, MI_WAVE);
+    k = (o > k) == up ? o : k;
+  }
+  static __device__ __forceinline__ void exchange(double& x, int& i, int step, bool up) {
+    const double ox = __shfl_xor(x, step, MI_WAVE);
+    const int oi = __shfl_xor(i, step, MI_WAVE);
+    const bool take = before(ox, oi, x, i) == up;
+    x = take ? ox : x;
+    i = take ? oi : i;
+  }
+  // the better of the list's and the newcomers' (x, i), best first
+  static __device__ __forceinline__ void merge(float& x, int& i, float nx, int ni, int lane) {
+    uint64_t n = key_of(nx, ni), own = key_of(x, i);
+#pragma unroll
+    for (int k = 2; k <= MI_WAVE; k <<= 1)
+#pragma unroll
+      for (int step = k >> 1; step > 0; step >>= 1) exchange(n, step, ((lane & k) == 0) == ((lane & step) == 0));
+    // of the list, and of the newcomers in rising order, the better one lane by lane: the best 64, falling, then rising
+    const uint64_t r = (uint64_t)(uint32_t)__shfl((int)(n >> 32), MI_WAVE - 1 - lane, MI_WAVE) << 32 |
+                       (uint32_t)__shfl((int)n, MI_WAVE - 1 - lane, MI_WAVE);
+    own = r > own ? r : own;
+#pragma unroll
+    for (int step = MI_WAVE / 2; step > 0; step >>= 1) exchange(own, step, (lane & step) == 0);
+    const uint32_t u = (uint32_t)(own >> 32);
+    x = __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+    i = ~(int)own;
+  }
+  static __device__ __forceinline__ void merge(double& x, int& i, double nx, int ni, int lane) {
+#pragma unroll
+    for (int k = 2; k <= MI_WAVE; k <<= 1)
+#pragma unroll
+      for (int step = k >> 1; step > 0; step >>= 1) exchange(nx, ni, step, ((lane & k) == 0) == ((lane & step) == 0));
+    const double rx = __shfl(nx, MI_WAVE - 1 - lane, MI_WAVE);
+    const int ri = __shfl(ni, MI_WAVE - 1 - lane, MI_WAVE);
+    const bool newer = before(rx, ri, x, i);
+    x = newer ? rx : x;
+    i = newer ? ri : i;
+#pragma unroll
+    for (int step = MI_WAVE / 2; step > 0; step >>= 1) exchange(x, i, step, (lane & step) == 0);
+  }
+  // one candidate of every lane (`real` of them)
+  __device__ __forceinline__ void take(X nx, int ni, bool real, int lane) {
+    const uint64_t mask = __ballot(real & before(nx, ni, last_x, last_i));
+    if ((mask >> lane) & 1) {
+      const int at = waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+      wait_x[at] = nx;
+      wait_i[at] = ni;
+    }
+    waiting += __builtin_popcountll(mask);
+  }
+  // those that wait, as far as they are whole 64s or, with `all`, to the last
+  __device__ __forceinline__ void join(int lane, bool all) {
+    int from = 0;
+    for (; waiting - from >= MI_WAVE || (all && waiting > from); from += MI_WAVE) {
+      X nx = -INFINITY;
+      int ni = INT32_MAX;
+      if (from + lane < waiting) {
+        nx = wait_x[from + lane];
+        ni = wait_i[from + lane];
+      }
+      merge(x, i, nx, ni, lane);
       last_x = lane_value(x, count - 1);
       last_i = __builtin_amdgcn_readlane(i, count - 1);
-      mask &= mask - 1;
-      mask &= __ballot(before(nx, ni, last_x, last_i));
+    }
+    if (from) {                        // the rest, fewer than 64, moves to the front
+      waiting = max(waiting - from, 0);
+      if (lane < waiting) {
+        const X rx = wait_x[from + lane];
+        const int ri = wait_i[from + lane];
+        wait_x[lane] = rx;
+        wait_i[lane] = ri;
+      }
     }
   }
 };
@@ -106,22 +182,41 @@ __device__ __forceinline__ int joined_place(const X* xs, const int* is, int wave
   return place;
 }
 
-// e^d for d <= 0, to 1e-11 of its value: 2^n e^r, |r| <= ln 2 / 2, by the series of e^r up to r^9.
-__device__ __forceinline__ double exp_of(double d) {
-  const double t = fmax(d * 1.4426950408889634, -1100.0);       // (2^-1100 is 0)
-  const double n = __builtin_rint(t);
-  const double r = (t - n) * 0.6931471805599453;
-  double p = 1.0 / 362880;
-  p = fma(p, r, 1.0 / 40320);
-  p = fma(p, r, 1.0 / 5040);
-  p = fma(p, r, 1.0 / 720);
-  p = fma(p, r, 1.0 / 120);
-  p = fma(p, r, 1.0 / 24);
-  p = fma(p, r, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return __builtin_ldexp(p, (int)n);
+// e^d for d <= 0, to 3e-12 of its value: with t = d / ln 2, n the whole number next to it and f = t - n, 2^n 2^f;
+// 2^f = 1 + f q(f), where q interpolates at the eight Chebyshev points of [-1/2, 1/2], so e^0 is 1.  The coefficients sit
+// in scalar registers, which the multiply-adds take as they are (constants are copied into vector registers before each).
+struct Exponential {
+  double c[8];
+  __device__ __forceinline__ Exponential()
+      : c{0.6931471805568324, 0.2402265069588842, 0.05550410906325485, 0.009618129135261179, 0.0013333478474028277,
+          0.0001540347517242934, 1.5303700625385598e-05, 1.3250807607943917e-06} {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+s"(c[i]));
+  }
+  __device__ __forceinline__ double operator()(double d) const {
+    const double t = fmax(d * 1.4426950408889634, -1100.0);       // (2^-1100 is 0)
+    const double n = __builtin_rint(t), f = t - n;
+    double p = fma(c[7], f, c[6]);
+#pragma unroll
+    for (int i = 5; i >= 0; --i) p = fma(p, f, c[i]);
+    return __builtin_ldexp(fma(p, f, 1.0), (int)n);
+  }
+};
+
+// The 16 logits of a lane in the tile at `at`: pieces of 4 side by side, -inf past the row's end.
+__device__ __forceinline__ void load_tile(const float* __restrict__ row, int64_t at, int V, int lane, f32x4 (&x)[4]) {
+  if (at + BEAM_TILE <= V) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const f32x4_any*>(row + at + (j * MI_WAVE + lane) * 4);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int64_t e = at + (j * MI_WAVE + lane) * 4 + c;
+        x[j][c] = e < V ? row[e] : -INFINITY;
+      }
+  }
 }
 
 struct BeamParts {
@@ -136,41 +231,49 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_rows_kernel(const float* __
                                                                  int count, int parts, int tiles, BeamParts out) {
   __shared__ float xs[BEAM_WAVES * BEAM_MAX_COUNT];
   __shared__ int is[BEAM_WAVES * BEAM_MAX_COUNT];
+  __shared__ float wait_x[BEAM_WAVES][BEAM_TILE + MI_WAVE];
+  __shared__ int wait_i[BEAM_WAVES][BEAM_TILE + MI_WAVE];
   __shared__ float maxima[BEAM_WAVES];
   __shared__ double sums[BEAM_WAVES];
-  const int lane = threadIdx.x & (MI_WAVE - 1), wave = threadIdx.x / MI_WAVE;
+  const int lane = threadIdx.x & (MI_WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / MI_WAVE);
   const int64_t r = blockIdx.x / parts;
   const int part = blockIdx.x % parts;
   const float* row = logits + r * row_stride;
-  Best<float> best(count);
+  const Exponential exp_of;
+  Best<float> best(count, wait_x[wave], wait_i[wave]);
   float m = -INFINITY;
   double s = 0.0;
-  // the part's tiles go round the waves
+  // The part's tiles go round the waves.  Which lane adds up a logit follows from its index alone: equal rows have equal
+  // sums wherever they lie.
   const int64_t first = ((int64_t)part * tiles * BEAM_WAVES + wave) * BEAM_TILE;
+  constexpr int64_t step = BEAM_WAVES * BEAM_TILE;
+  f32x4 next[4];
+  if (first < V) load_tile(row, first, V, lane, next);
   for (int t = 0; t < tiles; ++t) {
-    const int64_t at = first + (int64_t)t * BEAM_WAVES * BEAM_TILE;
+    const int64_t at = first + t * step;
     if (at >= V) break;
     f32x4 x[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      // (which lane adds up a logit follows from its index alone: equal rows have equal sums wherever they lie)
-      const int64_t e = at + (j * MI_WAVE + lane) * 4;
-      if (e + 4 <= V) {
-        x[j] = *reinterpret_cast<const f32x4_any*>(row + e);
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) x[j][c] = e + c < V ? row[e + c] : -INFINITY;
-      }
-    }
     float top = -INFINITY;
+    bool nan = false;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        x[j][c] = x[j][c] == x[j][c] ? x[j][c] : -INFINITY;
-        top = fmaxf(top, x[j][c]);
+        x[j][c] = next[j][c];
+        nan |= x[j][c] != x[j][c];
       }
-    const float tile_top = wave_max(top);
+    if (__ballot(nan)) {                 // (counts as -inf)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[j][c] = x[j][c] == x[j][c] ? x[j][c] : -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) top = fmaxf(top, x[j][c]);
+    if (t + 1 < tiles && at + step < V) load_tile(row, at + step, V, lane, next);
+    const float tile_top = wave_top(top);
     if (tile_top > m) {
       s *= exp_of((double)m - (double)tile_top);
       m = tile_top;
@@ -186,17 +289,18 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_rows_kernel(const float* __
 #pragma unroll
         for (int c = 0; c < 4; ++c) s += exp_of((double)x[j][c] - (double)m);
     }
-    // the candidates: at first those that `count` lanes reach, then those that come before the last of the list
-    if (tile_top < best.last_x) continue;
-    const float floor_x = t == 0 ? reached_by(top, count) : -INFINITY;
+    // the candidates: of the first tile those that reach what `count` lanes reach, then those that come before the last
+    // of the list
+    const float bar = t == 0 ? reached_by(top, count) : best.last_x;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int64_t e = at + (j * MI_WAVE + lane) * 4 + c;
-        const bool real = e < V && x[j][c] >= floor_x;
-        best.take(real ? x[j][c] : -INFINITY, real ? (int)e : INT32_MAX, lane);
+        if (__ballot(x[j][c] >= bar) == 0) continue;
+        const int e = (int)at + (j * MI_WAVE + lane) * 4 + c;
+        best.take(x[j][c], e, (e < V) & (x[j][c] >= bar), lane);
       }
+    best.join(lane, t == 0 || t + 1 == tiles || at + step >= V);
   }
   if (lane < count) {
     xs[wave * count + lane] = best.x;
@@ -229,20 +333,24 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_rows_kernel(const float* __
 }
 
 // Block: a group.
-__global__ __launch_bounds__(BEAM_THREADS) void beam_pick_kernel(const float* __restrict__ logits, int64_t row_stride,
+template <int WAVES>
+__global__ __launch_bounds__(WAVES * MI_WAVE) void beam_pick_kernel(const float* __restrict__ logits, int64_t row_stride,
                                                                  const float* __restrict__ scores, BeamParts in, int beams,
                                                                  int count, int parts, int V, float* __restrict__ out_scores,
                                                                  int* __restrict__ out_beams, int* __restrict__ out_tokens) {
   __shared__ float row_max[BEAM_MAX_BEAMS];
   __shared__ double row_base[BEAM_MAX_BEAMS];      // scores[b] - log of the row's sum; NaN: no candidate above -inf
   __shared__ int special;                          // rows whose lists do not say it all
-  __shared__ double xs[BEAM_WAVES * BEAM_MAX_COUNT];
-  __shared__ int is[BEAM_WAVES * BEAM_MAX_COUNT];
-  const int lane = threadIdx.x & (MI_WAVE - 1), wave = threadIdx.x / MI_WAVE;
+  __shared__ double wait_x[WAVES][2 * MI_WAVE];
+  __shared__ int wait_i[WAVES][2 * MI_WAVE];
+  __shared__ double xs[WAVES * BEAM_MAX_COUNT];
+  __shared__ int is[WAVES * BEAM_MAX_COUNT];
+  const int lane = threadIdx.x & (MI_WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / MI_WAVE);
   const int64_t r0 = (int64_t)blockIdx.x * beams;
+  const Exponential exp_of;
   if (threadIdx.x == 0) special = 0;
   __syncthreads();
-  for (int b = wave; b < beams; b += BEAM_WAVES) {
+  for (int b = wave; b < beams; b += WAVES) {
     float m = -INFINITY;
     for (int p = lane; p < parts; p += MI_WAVE) m = fmaxf(m, in.max[(r0 + b) * parts + p]);
     m = wave_max(m);
@@ -262,39 +370,35 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_pick_kernel(const float* __
     }
   }
   __syncthreads();
-  Best<double> best(count);
+  Best<double> best(count, wait_x[wave], wait_i[wave]);
   const int lists = parts * count, n = beams * lists;
-  for (int c0 = wave * MI_WAVE; c0 < n; c0 += BEAM_THREADS) {
-    const int c = c0 + lane, b = min(c / lists, beams - 1);
+  // ...the lists, then, where one of the rows is special: of a row without a candidate above -inf its first tokens, as far
+  // as they can be wanted; of a row with infinite logits the first of its other tokens, whose score is -inf (at most
+  // `count` of the infinite ones come before them)
+  const int reach = min(2 * count, V), all = n + (special ? beams * reach : 0);
+  const int rounds = (all + WAVES * MI_WAVE - 1) / (WAVES * MI_WAVE);
+  for (int round = 0; round < rounds; ++round) {
+    const int c = (round * WAVES + wave) * MI_WAVE + lane;
+    const bool listed = c < n;
+    const int b = min(listed ? c / lists : (c - n) / reach, beams - 1);
     const double base = row_base[b];
     const float m = row_max[b];
     float x = -INFINITY;
-    int token = INT32_MAX;
-    if (c < n) {
-      x = in.x[r0 * lists + c];
-      token = in.token[r0 * lists + c];
-    }
-    const bool real = token != INT32_MAX && base == base && (m < INFINITY || x == INFINITY);
-    best.take(real ? (x == m ? base : (double)x - (double)m + base) : -INFINITY, real ? b * V + token : INT32_MAX, lane);
-  }
-  if (special) {
-    // A row without a candidate above -inf: its first tokens, as far as they can be wanted.  A row with infinite logits:
-    // the first of its other tokens, whose score is -inf (at most `count` of the infinite ones come before them).
-    const int reach = min(2 * count, V);
-    for (int c0 = wave * MI_WAVE; c0 < beams * reach; c0 += BEAM_THREADS) {
-      const int c = c0 + lane, b = min(c / reach, beams - 1), token = c % reach;
-      bool real = c < beams * reach;
-      if (real && row_base[b] == row_base[b]) real = row_max[b] == INFINITY && logits[(r0 + b) * row_stride + token] != INFINITY;
-      best.take(-INFINITY, real ? b * V + token : INT32_MAX, lane);
-    }
+    int token = listed ? in.token[r0 * lists + c] : (c - n) % reach;
+    if (listed) x = in.x[r0 * lists + c];
+    bool real;
+    if (listed) real = token != INT32_MAX && base == base && (m < INFINITY || x == INFINITY);
+    else real = c < all && (base != base || (m == INFINITY && logits[(r0 + b) * row_stride + token] != INFINITY));
+    best.take(!listed ? -INFINITY : x == m ? base : (double)x - (double)m + base, real ? b * V + token : INT32_MAX, real, lane);
+    best.join(lane, round + 1 == rounds);
   }
   if (lane < count) {
     xs[wave * count + lane] = best.x;
     is[wave * count + lane] = best.i;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < BEAM_WAVES * count; i += BEAM_THREADS) {
-    const int place = joined_place(xs, is, BEAM_WAVES, count, i / count, i % count);
+  for (int i = threadIdx.x; i < WAVES * count; i += WAVES * MI_WAVE) {
+    const int place = joined_place(xs, is, WAVES, count, i / count, i % count);
     if (place < count) {
       const int64_t to = (int64_t)blockIdx.x * count + place;
       out_scores[to] = (float)xs[i];
@@ -342,8 +446,12 @@ MI_EXPORT int mi_beam_select(const float* logits, int64_t row_stride, const floa
   p.token = (int*)(p.x + rows * parts * count);
   beam_rows_kernel<<<(uint32_t)(rows * parts), BEAM_THREADS, 0, stream>>>(logits, row_stride, V, count, parts, tiles, p);
   MI_CHECK_LAUNCH("beam rows");
-  beam_pick_kernel<<<groups, BEAM_THREADS, 0, stream>>>(logits, row_stride, scores, p, beams, count, parts, V, out_scores,
-                                                        out_beams, out_tokens);
+  if (beams * parts * count > BEAM_FEW)
+    beam_pick_kernel<16><<<groups, 16 * MI_WAVE, 0, stream>>>(logits, row_stride, scores, p, beams, count, parts, V, out_scores,
+                                                              out_beams, out_tokens);
+  else
+    beam_pick_kernel<4><<<groups, 4 * MI_WAVE, 0, stream>>>(logits, row_stride, scores, p, beams, count, parts, V, out_scores,
+                                                            out_beams, out_tokens);
   MI_CHECK_LAUNCH("beam pick");
   return 0;
 }
