@@ -6,7 +6,7 @@
 __version__ = "0.1.0"
 
 from .config import EngineConfig
-from .sampling import SamplingParams
+from .sampling import BeamSearchParams, SamplingParams
 
 
 def __getattr__(name):

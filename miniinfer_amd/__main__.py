@@ -60,7 +60,7 @@ def _engine(args):
 
 
 def cmd_generate(args) -> int:
-  from miniinfer_amd import SamplingParams
+  from miniinfer_amd import BeamSearchParams, SamplingParams
   prompts = []
   for s in args.prompt or []:
     prompts.append(s)
@@ -74,6 +74,16 @@ def cmd_generate(args) -> int:
     if not prompts:
       print("give --prompt, --prompt-ids or --num-prompts", file=sys.stderr)
       return 2
+    if args.beams:
+      if args.temperature is not None:
+        print("--beams searches for the most probable continuations: give no --temperature", file=sys.stderr)
+        return 2
+      found = engine.beam_search(prompts, BeamSearchParams(num_beams=args.beams, max_tokens=args.max_tokens,
+                                                           length_penalty=args.length_penalty, ignore_eos=args.ignore_eos))
+      for p, hyps in zip(prompts, found):
+        print(json.dumps({"prompt": p, **hyps[0]}))
+      return 0
+    args.temperature = 0.7 if args.temperature is None else args.temperature
     sp = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                         ignore_eos=args.ignore_eos)
     outs = engine.generate(prompts=prompts, sampling_params=sp, use_tqdm=not args.quiet)
@@ -140,7 +150,10 @@ def main(argv=None) -> int:
   g = sub.add_parser("generate", help="generate from prompts")
   _engine_args(g)
   g.add_argument("--max-tokens", type=int, default=64, help="most tokens to generate")
-  g.add_argument("--temperature", type=float, default=0.7, help="sampling temperature (0 = greedy)")
+  g.add_argument("--temperature", type=float, default=None, help="sampling temperature (0 = greedy; default 0.7)")
+  g.add_argument("--beams", type=int, default=0, help="beam search with that many beams instead of sampling")
+  g.add_argument("--length-penalty", type=float, default=1.0,
+                 help="with --beams: hypotheses are compared by log-probability / length ** this")
   g.add_argument("--top-k", type=int, default=0)
   g.add_argument("--top-p", type=float, default=1.0)
   g.add_argument("--ignore-eos", action="store_true")

@@ -43,7 +43,8 @@ SPREAD_EVERY = 33
 
 class PagePool:
   """Free list of page ids 1..num_pages (page 0 is a scratch page that is never handed out).
-  Pages freed last are handed out first, so reuse shows early."""
+  Pages freed last are handed out first, so reuse shows early.  A page may have several holders (`share`); it is free
+  again when the last of them has given it back."""
 
   def __init__(self, num_pages: int):
     if num_pages <= 0:
@@ -57,7 +58,7 @@ class PagePool:
     first = [p for p in range(1, num_pages + 1) if p % SPREAD_EVERY]
     last = [p for p in range(1, num_pages + 1) if p % SPREAD_EVERY == 0]
     self._free: List[int] = (first + last)[::-1]
-    self._held = bytearray(num_pages + 1)
+    self._held = [0] * (num_pages + 1)       # how many hold each page
 
   @property
   def num_free(self) -> int:
@@ -79,11 +80,24 @@ class PagePool:
         raise CacheError(f"page id {p} does not exist")
       if not self._held[p]:
         raise CacheError(f"page {p} freed twice")
-      self._held[p] = 0
-      self._free.append(p)
+      self._held[p] -= 1
+      if not self._held[p]:
+        self._free.append(p)
+
+  def share(self, pages: Sequence[int]) -> None:
+    """One more holder of each of these pages."""
+    for p in pages:
+      if p <= 0 or p > self.num_pages or not self._held[p]:
+        raise CacheError(f"page {p} is not held, so it cannot be shared")
+      self._held[p] += 1
 
   def held(self) -> List[int]:
-    return [p for p in range(1, self.num_pages + 1) if self._held[p]]
+    """Every held page, as many times as it is held."""
+    return [p for p in range(1, self.num_pages + 1) for _ in range(self._held[p])]
+
+  @property
+  def num_held(self) -> int:
+    return sum(1 for n in self._held if n)
 
 
 @dataclass
@@ -384,6 +398,61 @@ class CacheManager:
     self._free_slots.append(self._slot.pop(req))
     del self._length[req]
 
+  def fork(self, children: Sequence[Tuple[Hashable, Hashable]]) -> None:
+    """For every (parent, child): `child` becomes a request that stands where `parent` does.  It shares the parent's full
+    pages, which nobody writes any more, and has copies of its own of the page that the next token goes to and of the
+    rows of the fixed-size states.  All or nothing; the copies are queued on the current stream, one launch for each
+    cache group and one for the states."""
+    seen = set()
+    for parent, child in children:
+      if parent not in self._slot:
+        raise CacheError(f"request {parent!r} is not admitted, so it cannot be forked")
+      if child in self._slot or child in seen:
+        raise CacheError(f"request {child!r} is admitted already")
+      seen.add(child)
+    if len(seen) > len(self._free_slots):
+      raise OutOfSlots(f"{len(seen)} request slots wanted, {len(self._free_slots)} of {self.max_requests} are free")
+    for gi, g in enumerate(self.paged):
+      want = sum(1 for parent, _ in children if self._length[parent] % g.page_size)
+      if want > g.pool.num_free:
+        raise OutOfPages(f"forking needs {want} pages in cache group {gi}, {g.pool.num_free} are free")
+    slots: List[Tuple[int, int]] = []
+    pages: List[List[Tuple[int, int]]] = [[] for _ in self.paged]
+    for parent, child in children:
+      n = self._length[parent]
+      slot = self._free_slots.pop()
+      self._slot[child], self._length[child] = slot, n
+      slots.append((self._slot[parent], slot))
+      for gi, g in enumerate(self.paged):
+        full, rest = divmod(n, g.page_size)
+        table = g.tables[parent][:full]
+        g.pool.share([p for p in table if p != 0])
+        if rest:
+          own = g.pool.alloc(1)[0]
+          pages[gi].append((g.tables[parent][full], own))
+          table.append(own)
+        g.tables[child] = table
+    for g, moves in zip(self.paged, pages):
+      if g.k is not None:
+        self._copy_rows([g.k, g.v], moves)
+    states = [s.state for s in self.states if s.state is not None]
+    for i in range(0, len(states), 8):
+      self._copy_rows(states[i:i + 8], slots)
+
+  def _copy_rows(self, buffers: Sequence[torch.Tensor], moves: Sequence[Tuple[int, int]]) -> None:
+    """Row `from` to row `to` in every layer of the buffers, for every (from, to); no row is both."""
+    if not moves:
+      return
+    index = torch.tensor(list(zip(*moves)), dtype=torch.int32).to(self.device)
+    if self.device.type == "cuda":
+      from ..kernels import ops
+      for i in range(0, len(moves), ops.MOVE_ROWS_MAX):
+        ops.move_rows(buffers, index[0, i:i + ops.MOVE_ROWS_MAX], index[1, i:i + ops.MOVE_ROWS_MAX])
+    else:
+      src, dst = index.long()
+      for t in buffers:
+        t[:, dst] = t[:, src]
+
   def table(self, group: int, req) -> List[int]:
     return self.paged[group].tables[req]
 
@@ -392,15 +461,17 @@ class CacheManager:
 
   # ------------------------------------------------------------------ invariants (tests, debug)
   def check(self) -> None:
-    """No page lost, none held twice, none both free and held; slots likewise."""
+    """No page lost, every page in as many tables as hold it, none both free and held; slots likewise."""
     for gi, g in enumerate(self.paged):
-      held = [p for t in g.tables.values() for p in t if p != 0]
-      if len(held) != len(set(held)):
-        raise CacheError(f"group {gi}: a page is in two block tables")
-      if sorted(held) != g.pool.held():
-        raise CacheError(f"group {gi}: tables hold {sorted(held)}, the pool says {g.pool.held()}")
-      if len(held) + g.pool.num_free != g.pool.num_pages:
-        raise CacheError(f"group {gi}: {len(held)} held + {g.pool.num_free} free != {g.pool.num_pages}")
+      for req, t in g.tables.items():
+        own = [p for p in t if p != 0]
+        if len(own) != len(set(own)):
+          raise CacheError(f"group {gi}: a page is twice in the block table of {req!r}")
+      held = sorted(p for t in g.tables.values() for p in t if p != 0)
+      if held != g.pool.held():
+        raise CacheError(f"group {gi}: tables hold {held}, the pool says {g.pool.held()}")
+      if g.pool.num_held + g.pool.num_free != g.pool.num_pages:
+        raise CacheError(f"group {gi}: {g.pool.num_held} held + {g.pool.num_free} free != {g.pool.num_pages}")
       if len(set(g.pool._free)) != len(g.pool._free) or set(g.pool._free) & set(held):
         raise CacheError(f"group {gi}: free list is inconsistent")
     slots = list(self._slot.values())

@@ -58,6 +58,24 @@ class AttentionSpec:
 
 
 @dataclass(frozen=True)
+class LinearAttentionSpec:
+  """Linear attention with a decay for each kv head over a state of fixed size:
+  S_t = exp(log_decay) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t."""
+  hidden_size: int
+  num_heads: int
+  num_kv_heads: int
+  head_dim: int
+  scale: float
+  log_decay: Tuple[float, ...]       # one for each kv head, <= 0 (-inf: no memory)
+  position: Any = NoPositionSpec()   # RotarySpec | NoPositionSpec | another registered kind
+  qk_norm: Optional[NormSpec] = None  # per-head norm of q and k before the rotation
+  tensor_names: Tuple[str, ...] = ("q_proj", "k_proj", "v_proj", "o_proj", "q_norm", "k_norm")
+  qkv_bias: bool = False
+  o_bias: bool = False
+  kind: str = "linear_attention"
+
+
+@dataclass(frozen=True)
 class GatedMLPSpec:
   """down( act(x Wg^T) * (x Wu^T) )."""
   hidden_size: int

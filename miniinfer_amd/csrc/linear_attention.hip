@@ -28,8 +28,8 @@ template <typename T, int NR>   // NR: rows of the state that a thread holds
 __global__ __launch_bounds__(LA_THREADS) void la_recurrent_kernel(
     const T* __restrict__ q, int64_t q_stride, const T* __restrict__ k, int64_t k_stride, const T* __restrict__ v,
     int64_t v_stride, T* __restrict__ out, int64_t out_stride, float* __restrict__ state, int64_t state_stride,
-    int num_rows, const int* __restrict__ rows, const int* __restrict__ cu, int num_tokens, int nkv, int rep, int d,
-    const float* __restrict__ log_decay, float scale) {
+    int num_rows, int idle_row, const int* __restrict__ rows, const int* __restrict__ cu, int num_tokens, int nkv, int rep,
+    int d, const float* __restrict__ log_decay, float scale) {
   __shared__ float part[2][LA_THREADS / MI_WAVE][LA_COLS];
   const int h = blockIdx.x % nkv, slice = blockIdx.x / nkv, b = blockIdx.y;
   const int lo = cu ? min(max(cu[b], 0), num_tokens) : b;
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(LA_THREADS) void la_recurrent_kernel(
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     const int i = ty + r * LA_ROW_GROUPS;
-    s[r] = live && i < d ? *reinterpret_cast<const f32x4*>(s_at + (int64_t)i * d) : f32x4{0.f, 0.f, 0.f, 0.f};
+    s[r] = live && i < d && row != idle_row ? *reinterpret_cast<const f32x4*>(s_at + (int64_t)i * d) : f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const float a = decay_power(log_decay[h], 1);
   int turn = 0;
@@ -100,6 +100,7 @@ __global__ __launch_bounds__(LA_THREADS) void la_recurrent_kernel(
       turn ^= 1;
     }
   }
+  if (row == idle_row) return;
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     const int i = ty + r * LA_ROW_GROUPS;
@@ -110,14 +111,14 @@ __global__ __launch_bounds__(LA_THREADS) void la_recurrent_kernel(
 template <typename T>
 static void launch_recurrent(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                              int64_t v_stride, void* out, int64_t out_stride, float* state, int64_t state_stride,
-                             int num_rows, const int* rows, const int* cu, int num_tokens, int num_requests, int nq,
+                             int num_rows, int idle_row, const int* rows, const int* cu, int num_tokens, int num_requests, int nq,
                              int nkv, int d, const float* log_decay, float scale, hipStream_t stream) {
   const dim3 grid(nkv * ((d + LA_COLS - 1) / LA_COLS), num_requests);
   const int nr = (d + LA_ROW_GROUPS - 1) / LA_ROW_GROUPS;
 #define LAUNCH(N)                                                                                                     \
   la_recurrent_kernel<T, N><<<grid, LA_THREADS, 0, stream>>>((const T*)q, q_stride, (const T*)k, k_stride, (const T*)v, \
-                                                             v_stride, (T*)out, out_stride, state, state_stride, num_rows, rows, \
-                                                             cu, num_tokens, nkv, nq / nkv, d, log_decay, scale)
+                                                             v_stride, (T*)out, out_stride, state, state_stride, num_rows, idle_row, \
+                                                             rows, cu, num_tokens, nkv, nq / nkv, d, log_decay, scale)
   if (nr <= 2) LAUNCH(2);
   else if (nr <= 4) LAUNCH(4);
   else LAUNCH(8);
@@ -126,7 +127,7 @@ static void launch_recurrent(const void* q, int64_t q_stride, const void* k, int
 
 #define LA_ARGS                                                                                                       \
   int dtype, const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v, int64_t v_stride, void *out, \
-      int64_t out_stride, float *state, int64_t state_stride, int num_rows, const int *rows, const int *cu, int num_tokens, \
+      int64_t out_stride, float *state, int64_t state_stride, int num_rows, int idle_row, const int *rows, const int *cu, int num_tokens, \
       int num_requests, int nq, int nkv, int d, const float *log_decay, float scale
 
 static int check_sizes(int nq, int nkv, int d, int num_requests, int64_t state_stride) {
@@ -141,10 +142,10 @@ MI_EXPORT int mi_linear_attention_recurrent(LA_ARGS, hipStream_t stream) {
   if (check_sizes(nq, nkv, d, num_requests, state_stride)) return 1;
   if (num_requests == 0 || num_tokens == 0) return 0;
   if (dtype == MI_DTYPE_BF16)
-    launch_recurrent<bf16>(q, q_stride, k, k_stride, v, v_stride, out, out_stride, state, state_stride, num_rows, rows, cu,
+    launch_recurrent<bf16>(q, q_stride, k, k_stride, v, v_stride, out, out_stride, state, state_stride, num_rows, idle_row, rows, cu,
                            num_tokens, num_requests, nq, nkv, d, log_decay, scale, stream);
   else if (dtype == MI_DTYPE_F32)
-    launch_recurrent<float>(q, q_stride, k, k_stride, v, v_stride, out, out_stride, state, state_stride, num_rows, rows, cu,
+    launch_recurrent<float>(q, q_stride, k, k_stride, v, v_stride, out, out_stride, state, state_stride, num_rows, idle_row, rows, cu,
                             num_tokens, num_requests, nq, nkv, d, log_decay, scale, stream);
   else
     MI_FAIL("linear attention: dtype %d", dtype);
@@ -359,7 +360,7 @@ struct LinearAttention {
   const float* log_decay;
   float* work;                       // states at the segments' starts, [unit][nkv][d][d]
   int64_t q_stride, k_stride, v_stride, out_stride, state_stride;
-  int num_rows, num_tokens, num_requests, nkv, rep, d;
+  int num_rows, idle_row, num_tokens, num_requests, nkv, rep, d;
   int segment;                       // tokens of a segment; 0: every request is one
   float scale;
 };
@@ -455,13 +456,13 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
   f32x4 s[KT];
   float* const s_row = a.state + (int64_t)row * a.state_stride + (int64_t)h * d * d;
   float* const s_work = a.segment ? a.work + ((int64_t)unit * a.nkv + h) * d * d : nullptr;
-  const float* const s_from = segments > 1 ? s_work : s_row;
+  const float* const s_from = segments > 1 ? s_work : row == a.idle_row ? nullptr : s_row;
 #pragma unroll
   for (int t = 0; t < KT; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 16 * t + g4 + i, c = n0 + l16;
-      s[t][i] = !STATES && r < d && c < d ? s_from[(int64_t)r * d + c] : 0.f;
+      s[t][i] = !STATES && s_from && r < d && c < d ? s_from[(int64_t)r * d + c] : 0.f;
     }
 
   const T* const kp = (const T*)a.k + (int64_t)h * d;
@@ -724,7 +725,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     }
   }
 
-  float* const s_to = STATES ? s_work : segment == segments - 1 ? s_row : nullptr;
+  float* const s_to = STATES ? s_work : segment == segments - 1 && row != a.idle_row ? s_row : nullptr;
   if (s_to) {
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
@@ -747,7 +748,8 @@ __global__ __launch_bounds__(256) void la_scan_kernel(LinearAttention a) {
   if (segments <= 1 || i >= a.nkv * per_head || row < 0 || row >= a.num_rows) return;
   const int h = i / per_head;
   const float an = decay_power(a.log_decay[h], a.segment);
-  f32x4 s = *reinterpret_cast<const f32x4*>(a.state + (int64_t)row * a.state_stride + (int64_t)i * 4);
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (row != a.idle_row) s = *reinterpret_cast<const f32x4*>(a.state + (int64_t)row * a.state_stride + (int64_t)i * 4);
   const int64_t unit = (int64_t)a.nkv * a.d * a.d;
   float* w = a.work + (int64_t)first_unit(a, b) * unit + (int64_t)i * 4;
   for (int x = 0; x < segments; ++x, w += unit) {
@@ -806,7 +808,7 @@ MI_EXPORT int mi_linear_attention(LA_ARGS, int segment, float* work, hipStream_t
   MI_REQUIRE(segment >= 0 && segment % 64 == 0 && (segment == 0 || work), "linear attention: segments of %d tokens", segment);
   if (num_requests == 0 || num_tokens == 0) return 0;
   LinearAttention a = {q, k, v, out, state, rows, cu, log_decay, work, q_stride, k_stride, v_stride, out_stride, state_stride,
-                       num_rows, num_tokens, num_requests, nkv, nq / nkv, d, segment, scale};
+                       num_rows, idle_row, num_tokens, num_requests, nkv, nq / nkv, d, segment, scale};
   if (dtype == MI_DTYPE_BF16) {
     if (d <= 64) return launch_prompt<bf16, 64, 4, LA_C64, LA_PBUF64, 2>(a, stream);
     if (d <= 128) return launch_prompt<bf16, 128, 8, 64, 2, 2>(a, stream);

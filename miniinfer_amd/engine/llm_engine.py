@@ -28,7 +28,7 @@ from ..cache.manager import CacheManager
 from ..config import EngineConfig, load_model_config, model_spec_of
 from ..kernels import ops
 from ..kernels.tuning import tune_products
-from ..sampling import Sampler, SamplingParams, request_seed
+from ..sampling import BeamSearchParams, Sampler, SamplingParams, request_seed
 from ..weights import build_model, fill_random, load_weights
 from .runner import ModelRunner, StepEntry
 from .scheduler import Request, ScheduledStep, Scheduler
@@ -354,6 +354,37 @@ class LLMEngine:
       text = self.tokenizer.decode(r.outputs) if self.tokenizer is not None else ""
       results.append({"text": text, "token_ids": list(r.outputs), "request_id": rid, "finish_reason": r.finish_reason})
     return results
+
+  # ------------------------------------------------------------------ beam search
+  def beam_search(self, prompts, params: Optional[BeamSearchParams] = None) -> List[List[dict]]:
+    """The most probable continuations by beam search (prompts as in `generate`; not while other requests are unfinished).
+    Returns, for every prompt, its `num_return` best hypotheses as dicts with "text", "token_ids",
+    "cumulative_logprob", "score" (that over length ** length_penalty) and "finish_reason" ("eos", "stop" or
+    "length")."""
+    from .beam_search import BeamSearcher
+    if isinstance(prompts, str) or (len(prompts) > 0 and isinstance(prompts[0], int)):
+      prompts = [prompts]
+    params = params if params is not None else BeamSearchParams()
+    if not self.is_finished():
+      raise RuntimeError("beam_search while requests are unfinished: run `step` until `is_finished`")
+    if params.num_beams > ops.BEAM_MAX_COUNT // 2:
+      raise ValueError(f"num_beams={params.num_beams}, at most {ops.BEAM_MAX_COUNT // 2} are supported")
+    V = self.model.spec.vocab_size
+    ids = [self._encode(p) for p in prompts]
+    for p in ids:
+      if not p:
+        raise ValueError("a beam search needs at least one prompt token")
+      if any(t < 0 or t >= V for t in p):
+        raise ValueError(f"prompt holds a token id outside [0, {V})")
+      if len(p) + params.max_tokens > self.max_model_len:
+        raise ValueError(f"prompt of {len(p)} tokens plus max_tokens={params.max_tokens} exceeds "
+                         f"max_model_len={self.max_model_len}")
+    out = []
+    for s in BeamSearcher(self, params).run(ids):
+      out.append([{"text": self.tokenizer.decode(h.tokens) if self.tokenizer is not None else "", "token_ids": list(h.tokens),
+                   "cumulative_logprob": h.score, "score": h.penalised, "finish_reason": h.reason}
+                  for h in s.finished[:params.num_return]])
+    return out
 
   def stream_generate(self, prompts, sampling_params: Union[SamplingParams, Sequence[SamplingParams], None] = None):
     """The same requests, yielded token by token as they are booked: a `RequestOutput` for every new token of

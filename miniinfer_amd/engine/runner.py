@@ -313,7 +313,8 @@ class ModelRunner:
     self.future_tokens = torch.zeros(max(1, cache.max_requests), dtype=torch.int32, device=self.device)
     if self.device.type == "cuda":
       from ..kernels import prepare
-      prepare(cache.dtype, [g.need.head_dim for g in cache.paged])      # what is not built yet, side by side
+      prepare(cache.dtype, [g.need.head_dim for g in cache.paged],      # what is not built yet, side by side
+              model.all_kernel_modules())
 
   def graph_pool(self):
     if self._graph_pool is None:

@@ -30,12 +30,12 @@ def build_all(force: bool = False) -> List[str]:
   return paths
 
 
-def prepare(dtype, head_dims) -> List[str]:
-  """Builds, side by side, the shared objects that a model of this dtype and these head sizes loads and that are not
-  built yet; returns what it built.  Each would otherwise be built at its first use, one after the other (a fresh
+def prepare(dtype, head_dims, modules=()) -> List[str]:
+  """Builds, side by side, the shared objects that a model of this dtype and these head sizes loads (and those of
+  `modules`) and that are not built yet; returns what it built.  Each would otherwise be built at its first use, one after the other (a fresh
   checkout's first step: about two minutes; side by side: as long as the slowest, half a minute)."""
   import torch
-  jobs = [("elementwise", ()), ("sampling", ()), ("gemm", ()), ("attention", ())]
+  jobs = [("elementwise", ()), ("sampling", ()), ("gemm", ()), ("attention", ())] + [(m, ()) for m in modules]
   if dtype == torch.bfloat16:
     jobs += [("gemm_skinny", ()), ("gemm_skinny", (("SKINNY_NT", 1),))]
     jobs += [("attention_mfma", (("HEAD_DIM", int(d)),)) for d in sorted(set(head_dims)) if d % 16 == 0 and 16 <= d <= 256]

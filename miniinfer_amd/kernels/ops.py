@@ -170,9 +170,9 @@ _SIGS["probes"] = {
 
 _SIGS["linear_attention"] = {
   "mi_linear_attention_recurrent": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
-                                    c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_float,
+                                    c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_float,
                                     c_void_p],
-  "mi_linear_attention": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int,
+  "mi_linear_attention": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int,
                           c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_float, c_int, c_void_p, c_void_p],
 }
 
@@ -1158,7 +1158,7 @@ def _linear_attention_rows(what, name, t, T, columns, dtype):
   return t.data_ptr(), stride[0]
 
 
-def _linear_attention_call(what, q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay, scale):
+def _linear_attention_call(what, q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay, scale, idle_row):
   """The checked arguments of a launch, as its entry points take them."""
   if nkv < 1 or nq < nkv or nq % nkv:
     raise KernelError(f"{what}: {nq} query heads are no multiple of {nkv} kv heads")
@@ -1187,7 +1187,8 @@ def _linear_attention_call(what, q, k, v, nq, nkv, d, out, state, state_rows, cu
   _i32("state_rows", state_rows)
   if log_decay.dtype is not torch.float32 or log_decay.numel() != nkv or not log_decay.is_contiguous():
     _f32("log_decay", log_decay, nkv)
-  return (code, qp, qs, kp, ks, vp, vs, op, os, sp, ss, shape[0], state_rows.data_ptr(), _ptr(cu_q), T, state_rows.numel(),
+  return (code, qp, qs, kp, ks, vp, vs, op, os, sp, ss, shape[0], -1 if idle_row is None else idle_row,
+          state_rows.data_ptr(), _ptr(cu_q), T, state_rows.numel(),
           nq, nkv, d, log_decay.data_ptr(), scale)
 
 
@@ -1204,21 +1205,23 @@ def linear_attention_segment(num_tokens: int, max_len: int, nkv: int, d: int, un
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int, nkv: int, d: int, out: torch.Tensor,
                      state: torch.Tensor, state_rows: torch.Tensor, cu_q: torch.Tensor, log_decay: torch.Tensor,
-                     scale: float, max_len: Optional[int] = None) -> torch.Tensor:
+                     scale: float, max_len: Optional[int] = None, idle_row: Optional[int] = None) -> torch.Tensor:
   """Linear attention with a decay for each head over the tokens of several requests, each going on from its state:
 
       S_t = a S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t,   a = exp(log_decay[kv head])
 
   q [T, >= nq*d], k, v [T, >= nkv*d] rows (the parts of a fused q|k|v buffer are fine), out [T, nq*d]; nq / nkv query
   heads share a kv head's state.  state float32 [rows, nkv, d, d] (key dim, value dim) is read at state_rows[b] and left
-  there as it is after request b's last token; requests of one call have rows of their own.  cu_q int32 [B + 1] = first
+  there as it is after request b's last token; requests of one call have rows of their own.  idle_row: a row that stands
+  for none; requests on it, any number, start from zeros and leave nothing (the padding entries of captured steps).  cu_q int32 [B + 1] = first
   token of each request: a request without tokens leaves its state as it is, rows of `out` that belong to no request are
   left as they are, and a state row outside the buffer gives rows of NaN.  log_decay float32 [nkv], <= 0 (-inf: a = 0)
   or positive for a growing state.  max_len: the most tokens of one request if the host knows it (default: T); it only
   chooses how the work is cut.  float32 and bfloat16; states and sums are 32-bit."""
-  args = _linear_attention_call("linear_attention", q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay, scale)
+  args = _linear_attention_call("linear_attention", q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay, scale,
+                                idle_row)
   _i32("cu_q", cu_q)
-  T = args[14]
+  T = args[15]
   if cu_q.numel() != state_rows.numel() + 1:
     raise KernelError(f"linear_attention: cu_q has {cu_q.numel()} entries for {state_rows.numel()} requests")
   with _on_device_of("linear_attention", q, k, v, out, state, state_rows, cu_q, log_decay) as stream:
@@ -1233,12 +1236,12 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int,
 
 def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int, nkv: int, d: int, out: torch.Tensor,
                           state: torch.Tensor, state_rows: torch.Tensor, log_decay: torch.Tensor,
-                          scale: float) -> torch.Tensor:
-  """`linear_attention` of one token for each request: row b of q, k, v and out is request b's token.  Requests may share
-  a state row that nobody reads afterwards (the padding entries of a captured step do)."""
-  args = _linear_attention_call("linear_attention_step", q, k, v, nq, nkv, d, out, state, state_rows, None, log_decay, scale)
-  if args[15] != args[14]:
-    raise KernelError(f"linear_attention_step: {args[15]} state rows for {args[14]} tokens")
+                          scale: float, idle_row: Optional[int] = None) -> torch.Tensor:
+  """`linear_attention` of one token for each request: row b of q, k, v and out is request b's token."""
+  args = _linear_attention_call("linear_attention_step", q, k, v, nq, nkv, d, out, state, state_rows, None, log_decay,
+                                scale, idle_row)
+  if args[16] != args[15]:
+    raise KernelError(f"linear_attention_step: {args[16]} state rows for {args[15]} tokens")
   with _on_device_of("linear_attention_step", q, k, v, out, state, state_rows, log_decay) as stream:
     lib = _lib("linear_attention")
     _check(lib, lib.mi_linear_attention_recurrent(*args, stream))

@@ -30,7 +30,7 @@ class PagedAttention(Part):
     self.nq, self.nkv, self.d = spec.num_heads, spec.num_kv_heads, spec.head_dim
     self.hidden = spec.hidden_size
     self.scale = float(spec.scale)
-    self.window = spec.window
+    self.window = getattr(spec, "window", None)
     self.position = POSITIONS.build(spec.position, ctx)
     self.q_norm = NORMS.build(spec.qk_norm, ctx) if spec.qk_norm is not None else None
     self.k_norm = NORMS.build(spec.qk_norm, ctx) if spec.qk_norm is not None else None

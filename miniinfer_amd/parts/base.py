@@ -107,6 +107,15 @@ class Part:
   # part are never captured.
   capturable = True
 
+  # kernel modules that the part launches beside those every model loads (`kernels.prepare` builds them ahead)
+  kernel_modules: Tuple[str, ...] = ()
+
+  def all_kernel_modules(self) -> List[str]:
+    out = set(self.kernel_modules)
+    for _, child in self.children():
+      out.update(child.all_kernel_modules())
+    return sorted(out)
+
   def is_capturable(self) -> bool:
     return bool(self.capturable) and all(child.is_capturable() for _, child in self.children())
 

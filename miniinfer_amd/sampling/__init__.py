@@ -1,2 +1,2 @@
-from .params import SamplingParams
+from .params import BeamSearchParams, SamplingParams
 from .sampler import Sampler, request_seed

@@ -33,3 +33,28 @@ class SamplingParams:
     self.stop_token_ids = [int(t) for t in (self.stop_token_ids or [])]
     if any(t < 0 for t in self.stop_token_ids):
       raise ValueError("stop_token_ids must be >= 0")
+
+
+@dataclass
+class BeamSearchParams:
+  """Options of `LLMEngine.beam_search`.  A hypothesis' score is its sum of log-probabilities divided by
+  length ** length_penalty, its length counted in generated tokens."""
+  num_beams: int = 4
+  max_tokens: int = 16
+  length_penalty: float = 1.0
+  early_stopping: bool = False  # True: a search ends with its num_beams-th finished hypothesis; False: when no running
+                                # beam scores better than the worst of them
+  num_return: int = 1           # hypotheses returned for each prompt, best first
+  ignore_eos: bool = False
+  stop_token_ids: List[int] = field(default_factory=list)   # end a hypothesis like the end-of-sequence token does
+
+  def __post_init__(self):
+    if self.num_beams <= 0:
+      raise ValueError("num_beams must be > 0")
+    if self.max_tokens <= 0:
+      raise ValueError("max_tokens must be > 0")
+    if not 1 <= self.num_return <= self.num_beams:
+      raise ValueError("num_return must be between 1 and num_beams")
+    self.stop_token_ids = [int(t) for t in (self.stop_token_ids or [])]
+    if any(t < 0 for t in self.stop_token_ids):
+      raise ValueError("stop_token_ids must be >= 0")

@@ -194,6 +194,32 @@ def test_linear_attention_with_a_state_row_that_does_not_exist(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lens", [[100, 3, 40, 70], [1, 600, 3, 400]])
+def test_requests_on_the_idle_row_start_from_nothing_and_leave_nothing(dtype, lens):
+  """Any number of them in a call, beside requests with states of their own, whole and in segments."""
+  from miniinfer_amd.kernels import ops
+  c = _Call(dtype, 4, 2, 64, lens, seed=31)
+  idle = c.state.shape[0] - 1
+  c.rows = [0, idle, 1, idle]
+  c.state[idle] = float("nan")                      # nobody reads it
+  qkv, state, rows, cu, g = c.device()
+  out = torch.full((c.T, 4 * 64), 7.0, dtype=dtype, device=DEV)
+  ops.linear_attention(*c.parts(qkv), 4, 2, 64, out, state, rows, cu, g, c.scale, idle_row=idle)
+  assert bool(state[idle].isnan().all())
+  # the same with a row of zeros for each
+  alone = _Call(dtype, 4, 2, 64, lens, seed=31)
+  alone.rows = [0, 2, 1, 3]
+  alone.state = c.state.clone()
+  alone.state[2:4] = 0.0
+  alone.state = alone.state[:4]
+  got = torch.cat([state[:2].cpu(), alone.run()[1][2:4]])
+  alone.check(out.cpu(), got)
+  step = torch.full((4, 4 * 64), 7.0, dtype=dtype, device=DEV)
+  ops.linear_attention_step(*c.parts(qkv[:4]), 4, 2, 64, step, state, rows, g, c.scale, idle_row=idle)
+  assert bool(step.isfinite().all()) and bool(state[idle].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_linear_attention_with_strides(dtype):
   """Rows of q, k, v and out in wider buffers at odd offsets, states in every second row of a larger buffer."""
   from miniinfer_amd.kernels import ops
