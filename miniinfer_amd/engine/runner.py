@@ -314,7 +314,7 @@ class ModelRunner:
     if self.device.type == "cuda":
       from ..kernels import prepare
       prepare(cache.dtype, [g.need.head_dim for g in cache.paged],      # what is not built yet, side by side
-              model.all_kernel_modules())
+              getattr(model, "all_kernel_modules", list)())
 
   def graph_pool(self):
     if self._graph_pool is None:
