@@ -66,19 +66,17 @@ static void launch_move_rows(RowBuffers& bufs, const int* src, const int* dst, i
   move_rows_kernel<P, THREADS><<<(uint32_t)blocks, THREADS, 0, stream>>>(bufs, src, dst, moves, wide);
 }
 
-// base, layer_bytes, row_stride, row_bytes, layers, rows: `count` of each, on the host.
-MI_EXPORT int mi_move_rows(int count, void* const* base, const int64_t* layer_bytes, const int64_t* row_stride,
-                           const int64_t* row_bytes, const int* layers, const int* rows, const int* src, const int* dst,
-                           int moves, hipStream_t stream) {
+// spec: of each of the `count` buffers, on the host, its address, the bytes from layer to layer, from row to row and of a
+// row, its layers and rows.
+MI_EXPORT int mi_move_rows(int count, const int64_t* spec, const int* src, const int* dst, int moves, hipStream_t stream) {
   MI_REQUIRE(count >= 1 && count <= ROWS_MAX_BUFFERS, "move_rows: %d buffers, 1 to %d are taken", count, ROWS_MAX_BUFFERS);
-  MI_REQUIRE(moves >= 0 && moves <= ROWS_MAX_MOVES, "move_rows: %d moves, at most %d are taken", moves,
-             ROWS_MAX_MOVES);
+  MI_REQUIRE(moves >= 0 && moves <= ROWS_MAX_MOVES, "move_rows: %d moves, at most %d are taken", moves, ROWS_MAX_MOVES);
   if (moves == 0) return 0;
   uint64_t align = 0;
   for (int b = 0; b < count; ++b) {
-    MI_REQUIRE(layers[b] >= 0 && rows[b] >= 0 && row_bytes[b] >= 0 && row_stride[b] >= row_bytes[b],
-               "move_rows: bad sizes of buffer %d", b);
-    align |= (uint64_t)base[b] | (uint64_t)layer_bytes[b] | (uint64_t)row_stride[b] | (uint64_t)row_bytes[b];
+    const int64_t* s = spec + 6 * b;
+    MI_REQUIRE(s[3] >= 0 && s[2] >= s[3] && s[4] >= 0 && s[5] >= 0 && s[5] <= INT32_MAX, "move_rows: bad sizes of buffer %d", b);
+    align |= (uint64_t)s[0] | (uint64_t)s[1] | (uint64_t)s[2] | (uint64_t)s[3];
   }
   const int piece = align % 16 == 0 ? 16 : align % 4 == 0 ? 4 : align % 2 == 0 ? 2 : 1;
   // Columns to a workgroup: as many as its registers hold for all moves.
@@ -90,13 +88,14 @@ MI_EXPORT int mi_move_rows(int count, void* const* base, const int64_t* layer_by
   bufs.count = count;
   int64_t blocks = 0;
   for (int b = 0; b < count; ++b) {
-    bufs.base[b] = (char*)base[b];
-    bufs.layer_bytes[b] = layer_bytes[b];
-    bufs.row_stride[b] = row_stride[b];
-    bufs.pieces[b] = row_bytes[b] / piece;
-    bufs.rows[b] = rows[b];
+    const int64_t* s = spec + 6 * b;
+    bufs.base[b] = (char*)s[0];
+    bufs.layer_bytes[b] = s[1];
+    bufs.row_stride[b] = s[2];
+    bufs.pieces[b] = s[3] / piece;
+    bufs.rows[b] = (int)s[5];
     bufs.first_block[b] = blocks;
-    blocks += (int64_t)layers[b] * ((bufs.pieces[b] + (1 << wide) - 1) >> wide);
+    blocks += s[4] * ((bufs.pieces[b] + (1 << wide) - 1) >> wide);
   }
   bufs.first_block[count] = blocks;
   MI_REQUIRE(blocks <= 0x7fffffff, "move_rows: %lld workgroups are too many for one launch", (long long)blocks);

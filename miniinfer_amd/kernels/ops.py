@@ -183,7 +183,7 @@ _SIGS["beam"] = {
 }
 
 _SIGS["rows"] = {
-  "mi_move_rows": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
+  "mi_move_rows": [c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
 }
 
 _RESULTS = {"mi_beam_scratch": c_int64}     # entry points that return something else than an int
@@ -512,9 +512,11 @@ _COMPUTE_UNITS: Dict[int, int] = {}
 def compute_units(device=None) -> int:
   """Compute units of the device (256 on an MI355X, which is also what is assumed where there is no GPU to ask, as in
   host-only tests of the launch rules).  The launch rules derive from it how many workgroups or waves fill the chip."""
+  if type(device) is int and device in _COMPUTE_UNITS:
+    return _COMPUTE_UNITS[device]
   if not torch.cuda.is_available():
     return 256
-  index = torch.device(device).index if device is not None else None
+  index = device if type(device) is int else torch.device(device).index if device is not None else None
   if index is None:
     index = torch.cuda.current_device()
   if index not in _COMPUTE_UNITS:
@@ -1226,7 +1228,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int,
     raise KernelError(f"linear_attention: cu_q has {cu_q.numel()} entries for {state_rows.numel()} requests")
   with _on_device_of("linear_attention", q, k, v, out, state, state_rows, cu_q, log_decay) as stream:
     lib = _lib("linear_attention")
-    segment = linear_attention_segment(T, T if max_len is None else min(max_len, T), nkv, d, compute_units(q.device))
+    segment = linear_attention_segment(T, T if max_len is None else min(max_len, T), nkv, d, compute_units(q.get_device()))
     work = None
     if segment:
       work = torch.empty((T // segment + state_rows.numel()) * nkv * d * d, dtype=torch.float32, device=q.device)
@@ -1281,7 +1283,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_beams: int,
                       f"{BEAM_MAX_BEAMS} beams are taken")
   with _on_device_of("beam_select", logits, scores) as stream:
     lib = _lib("beam")
-    units = compute_units(logits.device)
+    units = compute_units(logits.get_device())
     scratch = torch.empty(lib.mi_beam_scratch(G, num_beams, V, count, units), dtype=torch.float64, device=logits.device)
     out_scores = torch.empty((G, count), dtype=torch.float32, device=logits.device)
     beams, tokens = torch.empty((2, G, count), dtype=torch.int32, device=logits.device).unbind()
@@ -1302,43 +1304,44 @@ def move_rows(buffers, src: torch.Tensor, dst: torch.Tensor) -> None:
   tensor or up to 8 of them, [layers, rows, ...] with dense rows, of any dtype: a cache group's key and value pages, a
   group's states.  src, dst: int32 [n] on the device, n up to 16,384; entries outside a buffer's rows move nothing there
   (pad with -1)."""
-  if isinstance(buffers, torch.Tensor):
-    buffers = [buffers]
-  buffers = list(buffers)
+  buffers = [buffers] if isinstance(buffers, torch.Tensor) else list(buffers)
   if not 1 <= len(buffers) <= MOVE_ROWS_MAX_BUFFERS:
     raise KernelError(f"move_rows: {len(buffers)} buffers, 1 to {MOVE_ROWS_MAX_BUFFERS} are taken")
+  spec = []               # address, bytes from layer to layer, from row to row and of a row, layers, rows of each buffer
   for t in buffers:
-    if t.dim() < 2:
-      raise KernelError(f"move_rows: a buffer must be [layers, rows, ...], got {tuple(t.shape)}")
-    if not t[:1, :1].is_contiguous():
-      raise KernelError("move_rows: the rows of a buffer must be dense")
-    if t.numel():
-      extent = t[0, 0].numel()
-      for stride, n in sorted((t.stride(i), t.shape[i]) for i in (0, 1) if t.shape[i] > 1):
+    shape, total = t.shape, t.numel()
+    if len(shape) < 2:
+      raise KernelError(f"move_rows: a buffer must be [layers, rows, ...], got {tuple(shape)}")
+    if total == 0:
+      continue
+    layers, rows, size = shape[0], shape[1], t.element_size()
+    row = total // (layers * rows)
+    if t.is_contiguous():
+      per_layer, per_row = rows * row, row
+    else:
+      if not t[0, 0].is_contiguous():
+        raise KernelError("move_rows: the rows of a buffer must be dense")
+      extent = row
+      for stride, n in sorted((t.stride(i), shape[i]) for i in (0, 1) if shape[i] > 1):
         if stride < extent:
           raise KernelError(f"move_rows: rows or layers of a buffer overlap (strides {t.stride()})")
         extent += (n - 1) * stride
-  _i32("src", src)
-  _i32("dst", dst)
+      per_layer = t.stride(0) if layers > 1 else row
+      per_row = t.stride(1) if rows > 1 else row
+    spec += (t.data_ptr(), per_layer * size, per_row * size, row * size, layers, rows)
   n = src.numel()
+  if src.dtype is not torch.int32 or dst.dtype is not torch.int32 or not src.is_contiguous() or not dst.is_contiguous():
+    _i32("src", src)
+    _i32("dst", dst)
   if dst.numel() != n:
     raise KernelError(f"move_rows: {n} sources, {dst.numel()} destinations")
   if n > MOVE_ROWS_MAX:
     raise KernelError(f"move_rows: {n} moves, at most {MOVE_ROWS_MAX} are taken")
   with _on_device_of("move_rows", src, dst, *buffers) as stream:
-    lib = _lib("rows")
-    live = [t for t in buffers if t.numel()]
-    if n == 0 or not live:
+    if n == 0 or not spec:
       return
-    m = len(live)
-    size = [t.element_size() for t in live]
-    row = [t[0, 0].numel() * e for t, e in zip(live, size)]
-    stride1 = [t.stride(1) * e if t.shape[1] > 1 else r for t, e, r in zip(live, size, row)]
-    stride0 = [t.stride(0) * e if t.shape[0] > 1 else r for t, e, r in zip(live, size, row)]
-    i64, i32 = c_int64 * m, c_int * m
-    _check(lib, lib.mi_move_rows(m, (c_void_p * m)(*[_ptr(t) for t in live]), i64(*stride0), i64(*stride1), i64(*row),
-                                 i32(*[t.shape[0] for t in live]), i32(*[t.shape[1] for t in live]), _ptr(src), _ptr(dst), n,
-                                 stream))
+    lib = _lib("rows")
+    _check(lib, lib.mi_move_rows(len(spec) // 6, (c_int64 * len(spec))(*spec), src.data_ptr(), dst.data_ptr(), n, stream))
 
 
 # ----------------------------------------------------------------------------- what the device delivers
