@@ -12,8 +12,14 @@
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 #define ROWS_MAX_BUFFERS 8
-#define ROWS_PIECES 16           // pieces that a thread holds: 64 registers of 16-byte pieces
-#define ROWS_MAX_MOVES (1024 * ROWS_PIECES)
+// Pieces that a thread holds.  Few of them, in workgroups of 512 threads, keep more workgroups on a compute unit, some
+// loading while others store (12 layers of 64 states of 512 KB: 146 us, 4.5 TB/s; with 16 pieces in 256 threads 174);
+// long lists take what registers there are, so that a row's columns still come in whole lines.
+#define ROWS_PIECES 4
+#define ROWS_THREADS 512
+#define ROWS_PIECES_MANY 16
+#define ROWS_THREADS_MANY 1024
+#define ROWS_MAX_MOVES (ROWS_THREADS_MANY * ROWS_PIECES_MANY)
 
 struct RowBuffers {
   char* base[ROWS_MAX_BUFFERS];
@@ -26,7 +32,7 @@ struct RowBuffers {
 };
 
 // Thread t holds the pieces t, t + THREADS, ... of the (move, column) table of its workgroup, 1 << wide columns to a move.
-template <typename P, int THREADS>
+template <typename P, int THREADS, int PIECES>
 __global__ __launch_bounds__(THREADS) void move_rows_kernel(RowBuffers bufs, const int* __restrict__ src,
                                                             const int* __restrict__ dst, int moves, int wide) {
   int b = 0;
@@ -36,10 +42,10 @@ __global__ __launch_bounds__(THREADS) void move_rows_kernel(RowBuffers bufs, con
   const int64_t layer = block / spans, column0 = (block % spans) << wide;
   char* base = bufs.base[b] + layer * bufs.layer_bytes[b];
   const int rows = bufs.rows[b];
-  P held[ROWS_PIECES];
-  char* to[ROWS_PIECES];
+  P held[PIECES];
+  char* to[PIECES];
 #pragma unroll
-  for (int r = 0; r < ROWS_PIECES; ++r) {
+  for (int r = 0; r < PIECES; ++r) {
     const int i = threadIdx.x + r * THREADS;
     const int move = i >> wide;
     const int64_t column = column0 + (i & ((1 << wide) - 1));
@@ -56,14 +62,14 @@ __global__ __launch_bounds__(THREADS) void move_rows_kernel(RowBuffers bufs, con
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < ROWS_PIECES; ++r)
+  for (int r = 0; r < PIECES; ++r)
     if (to[r]) *reinterpret_cast<P*>(to[r]) = held[r];
 }
 
-template <typename P, int THREADS>
+template <typename P, int THREADS, int PIECES>
 static void launch_move_rows(RowBuffers& bufs, const int* src, const int* dst, int moves, int wide, int64_t blocks,
                              hipStream_t stream) {
-  move_rows_kernel<P, THREADS><<<(uint32_t)blocks, THREADS, 0, stream>>>(bufs, src, dst, moves, wide);
+  move_rows_kernel<P, THREADS, PIECES><<<(uint32_t)blocks, THREADS, 0, stream>>>(bufs, src, dst, moves, wide);
 }
 
 // spec: of each of the `count` buffers, on the host, its address, the bytes from layer to layer, from row to row and of a
@@ -80,8 +86,8 @@ MI_EXPORT int mi_move_rows(int count, const int64_t* spec, const int* src, const
   }
   const int piece = align % 16 == 0 ? 16 : align % 4 == 0 ? 4 : align % 2 == 0 ? 2 : 1;
   // Columns to a workgroup: as many as its registers hold for all moves.
-  const bool many = moves > 256 * ROWS_PIECES / 8;
-  const int room = (many ? 1024 : 256) * ROWS_PIECES;
+  const bool many = moves > ROWS_THREADS * ROWS_PIECES / 8;
+  const int room = many ? ROWS_THREADS_MANY * ROWS_PIECES_MANY : ROWS_THREADS * ROWS_PIECES;
   int wide = 0;
   while (wide < 12 && ((int64_t)moves << (wide + 1)) <= room) ++wide;
   RowBuffers bufs;
@@ -100,8 +106,8 @@ MI_EXPORT int mi_move_rows(int count, const int64_t* spec, const int* src, const
   bufs.first_block[count] = blocks;
   MI_REQUIRE(blocks <= 0x7fffffff, "move_rows: %lld workgroups are too many for one launch", (long long)blocks);
   if (blocks == 0) return 0;
-#define LAUNCH(P) (many ? launch_move_rows<P, 1024>(bufs, src, dst, moves, wide, blocks, stream) \
-                        : launch_move_rows<P, 256>(bufs, src, dst, moves, wide, blocks, stream))
+#define LAUNCH(P) (many ? launch_move_rows<P, ROWS_THREADS_MANY, ROWS_PIECES_MANY>(bufs, src, dst, moves, wide, blocks, stream) \
+                        : launch_move_rows<P, ROWS_THREADS, ROWS_PIECES>(bufs, src, dst, moves, wide, blocks, stream))
   if (piece == 16) LAUNCH(u32x4);
   else if (piece == 4) LAUNCH(uint32_t);
   else if (piece == 2) LAUNCH(uint16_t);
