@@ -169,7 +169,7 @@ _SIGS["probes"] = {
 }
 
 _SIGS["linear_attention"] = {
-  "mi_linear_attention_recurrent": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+  "mi_linear_attention_step": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
                                     c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_float,
                                     c_void_p],
   "mi_linear_attention": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int,
@@ -1246,7 +1246,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq:
     raise KernelError(f"linear_attention_step: {args[16]} state rows for {args[15]} tokens")
   with _on_device_of("linear_attention_step", q, k, v, out, state, state_rows, log_decay) as stream:
     lib = _lib("linear_attention")
-    _check(lib, lib.mi_linear_attention_recurrent(*args, stream))
+    _check(lib, lib.mi_linear_attention_step(*args, stream))
   return out
 
 

@@ -150,6 +150,13 @@ def test_linear_attention_step(dtype, nq, nkv, d):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_linear_attention_step_of_many_requests(dtype):
+  """So many states that they are read past the caches."""
+  c = _Call(dtype, 4, 2, 128, [1] * 530, seed=6)
+  c.check(*c.run(step=True))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("log_decay", [[float("-inf"), 0.0], [-30.0, -1e-6], [-200.0, 0.01]])
 def test_linear_attention_at_the_ends_of_the_decay(dtype, log_decay):
   """No memory at all, no forgetting, powers that leave the range of 32 bits, a state that grows."""
