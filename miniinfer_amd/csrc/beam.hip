@@ -32,17 +32,68 @@ __device__ __forceinline__ float lane_value(float x, int lane) { return __uint_a
 __device__ __forceinline__ double lane_value(double x, int lane) {
   return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), lane), __builtin_amdgcn_readlane(__double2loint(x), lane));
 }
-// The largest value of the wave, in a scalar register: four shifts within rows of 16 lanes, two broadcasts across rows.
-__device__ __forceinline__ float wave_top(float x) {
-#define STEP(CTRL, ROWS) x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), CTRL, ROWS, 0xf, false)))
-  STEP(0x111, 0xf);    // row_shr:1
-  STEP(0x112, 0xf);    // row_shr:2
-  STEP(0x114, 0xf);    // row_shr:4
-  STEP(0x118, 0xf);    // row_shr:8
-  STEP(0x142, 0xa);    // row_bcast:15 into rows 1 and 3
-  STEP(0x143, 0xc);    // row_bcast:31 into rows 2 and 3
-#undef STEP
-  return lane_value(x, 63);
+// The value of lane l ^ step, without a way through LDS: permutations within 4, 8 and 16 lanes, swaps of rows of 16 and of
+// halves of the wave.  `step`: a power of two, a constant where this is inlined.
+__device__ __forceinline__ int xor_lane(int x, int step, int lane) {
+#define PERMUTED(X, CTRL) __builtin_amdgcn_update_dpp(X, X, CTRL, 0xf, 0xf, false)
+  switch (step) {
+    case 1: return PERMUTED(x, 0xB1);                           // quad_perm [1, 0, 3, 2]
+    case 2: return PERMUTED(x, 0x4E);                           // quad_perm [2, 3, 0, 1]
+    case 4: {
+      const int y = PERMUTED(x, 0x141);                         // row_half_mirror: l ^ 7, then l ^ 3
+      return PERMUTED(y, 0x1B);                                 // quad_perm [3, 2, 1, 0]
+    }
+    case 8: return PERMUTED(x, 0x128);                          // row_ror:8
+    case 16: {
+      const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+      return (lane & 16) ? (int)r[0] : (int)r[1];
+    }
+    default: {
+      const auto r = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+      return (lane & 32) ? (int)r[0] : (int)r[1];
+    }
+  }
+}
+__device__ __forceinline__ float xor_lane(float x, int step, int lane) { return __int_as_float(xor_lane(__float_as_int(x), step, lane)); }
+__device__ __forceinline__ double xor_lane(double x, int step, int lane) {
+  return __hiloint2double(xor_lane(__double2hiint(x), step, lane), xor_lane(__double2loint(x), step, lane));
+}
+__device__ __forceinline__ uint64_t xor_lane(uint64_t x, int step, int lane) {
+  return (uint64_t)(uint32_t)xor_lane((int)(x >> 32), step, lane) << 32 | (uint32_t)xor_lane((int)x, step, lane);
+}
+// The value of lane 63 - l.
+__device__ __forceinline__ int mirrored(int x, int lane) {
+  return xor_lane(xor_lane(PERMUTED(x, 0x140), 16, lane), 32, lane);       // row_mirror
+}
+__device__ __forceinline__ double mirrored(double x, int lane) {
+  return __hiloint2double(mirrored(__double2hiint(x), lane), mirrored(__double2loint(x), lane));
+}
+__device__ __forceinline__ uint64_t mirrored(uint64_t x, int lane) {
+  return (uint64_t)(uint32_t)mirrored((int)(x >> 32), lane) << 32 | (uint32_t)mirrored((int)x, lane);
+}
+#undef PERMUTED
+__device__ __forceinline__ double sum_of_lanes(double x, int lane) {
+#pragma unroll
+  for (int step = 1; step < MI_WAVE; step <<= 1) x += xor_lane(x, step, lane);
+  return x;
+}
+// The largest value of the wave, in a scalar register.
+__device__ __forceinline__ float wave_top(float x, int lane) {
+#pragma unroll
+  for (int step = 1; step < MI_WAVE; step <<= 1) x = fmaxf(x, xor_lane(x, step, lane));
+  return lane_value(x, 0);
+}
+// What at least `count` of the lanes' values reach: the count-th largest of them (the lanes sorted, largest first, by a
+// bitonic network).
+__device__ __forceinline__ float reached_by(float x, int count, int lane) {
+#pragma unroll
+  for (int k = 2; k <= MI_WAVE; k <<= 1)
+#pragma unroll
+    for (int step = k >> 1; step > 0; step >>= 1) {
+      const float o = xor_lane(x, step, lane);
+      x = ((lane & k) == 0) == ((lane & step) == 0) ? fmaxf(x, o) : fminf(x, o);
+    }
+  return lane_value(x, count - 1);
 }
 
 // A wave's best candidates: lane l holds the l-th in order.  Newcomers that come before the last of the `count` that are
@@ -69,31 +120,30 @@ struct Best {
     const uint32_t u = __float_as_uint(x + 0.f);       // (-0 and 0 are equal)
     return (uint64_t)((u & 0x80000000u) ? ~u : (u | 0x80000000u)) << 32 | (uint32_t)~i;
   }
-  // the wave's candidates (x, i) and those of the lanes `step` away: the better one to the lanes where `up`
-  static __device__ __forceinline__ void exchange(uint64_t& k, int step, bool up) {
-    const uint64_t o = (uint64_t)(uint32_t)__shfl_xor((int)(k >> 32), step, MI_WAVE) << 32 | (uint32_t)__shfl_xor((int)k, step, MI_WAVE);
+  // the wave's candidates and those of the lanes `step` away: the better one to the lanes where `up`
+  static __device__ __forceinline__ void exchange(uint64_t& k, int step, bool up, int lane) {
+    const uint64_t o = xor_lane(k, step, lane);
     k = (o > k) == up ? o : k;
   }
-  static __device__ __forceinline__ void exchange(double& x, int& i, int step, bool up) {
-    const double ox = __shfl_xor(x, step, MI_WAVE);
-    const int oi = __shfl_xor(i, step, MI_WAVE);
+  static __device__ __forceinline__ void exchange(double& x, int& i, int step, bool up, int lane) {
+    const double ox = xor_lane(x, step, lane);
+    const int oi = xor_lane(i, step, lane);
     const bool take = before(ox, oi, x, i) == up;
     x = take ? ox : x;
     i = take ? oi : i;
   }
-  // the better of the list's and the newcomers' (x, i), best first
+  // The better of the list's and the newcomers' candidates, best first.  The newcomers are sorted; of the list, and of
+  // the newcomers in rising order, the better one lane by lane are the best 64, falling, then rising; merged.
   static __device__ __forceinline__ void merge(float& x, int& i, float nx, int ni, int lane) {
     uint64_t n = key_of(nx, ni), own = key_of(x, i);
 #pragma unroll
     for (int k = 2; k <= MI_WAVE; k <<= 1)
 #pragma unroll
-      for (int step = k >> 1; step > 0; step >>= 1) exchange(n, step, ((lane & k) == 0) == ((lane & step) == 0));
-    // of the list, and of the newcomers in rising order, the better one lane by lane: the best 64, falling, then rising
-    const uint64_t r = (uint64_t)(uint32_t)__shfl((int)(n >> 32), MI_WAVE - 1 - lane, MI_WAVE) << 32 |
-                       (uint32_t)__shfl((int)n, MI_WAVE - 1 - lane, MI_WAVE);
+      for (int step = k >> 1; step > 0; step >>= 1) exchange(n, step, ((lane & k) == 0) == ((lane & step) == 0), lane);
+    const uint64_t r = mirrored(n, lane);
     own = r > own ? r : own;
 #pragma unroll
-    for (int step = MI_WAVE / 2; step > 0; step >>= 1) exchange(own, step, (lane & step) == 0);
+    for (int step = MI_WAVE / 2; step > 0; step >>= 1) exchange(own, step, (lane & step) == 0, lane);
     const uint32_t u = (uint32_t)(own >> 32);
     x = __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
     i = ~(int)own;
@@ -102,14 +152,14 @@ struct Best {
 #pragma unroll
     for (int k = 2; k <= MI_WAVE; k <<= 1)
 #pragma unroll
-      for (int step = k >> 1; step > 0; step >>= 1) exchange(nx, ni, step, ((lane & k) == 0) == ((lane & step) == 0));
-    const double rx = __shfl(nx, MI_WAVE - 1 - lane, MI_WAVE);
-    const int ri = __shfl(ni, MI_WAVE - 1 - lane, MI_WAVE);
+      for (int step = k >> 1; step > 0; step >>= 1) exchange(nx, ni, step, ((lane & k) == 0) == ((lane & step) == 0), lane);
+    const double rx = mirrored(nx, lane);
+    const int ri = mirrored(ni, lane);
     const bool newer = before(rx, ri, x, i);
     x = newer ? rx : x;
     i = newer ? ri : i;
 #pragma unroll
-    for (int step = MI_WAVE / 2; step > 0; step >>= 1) exchange(x, i, step, (lane & step) == 0);
+    for (int step = MI_WAVE / 2; step > 0; step >>= 1) exchange(x, i, step, (lane & step) == 0, lane);
   }
   // one candidate of every lane (`real` of them)
   __device__ __forceinline__ void take(X nx, int ni, bool real, int lane) {
@@ -146,18 +196,6 @@ struct Best {
     }
   }
 };
-
-// What at least `count` of the lanes' values reach: the count-th largest of them.
-template <typename X>
-__device__ __forceinline__ X reached_by(X x, int count) {
-  int above = 0;
-  for (int l = 0; l < MI_WAVE; ++l) {
-    const X y = lane_value(x, l);
-    above += (y > x || (y == x && l < (int)(threadIdx.x & (MI_WAVE - 1)))) ? 1 : 0;
-  }
-  const uint64_t mask = __ballot(above == count - 1);
-  return lane_value(x, mask ? __builtin_ctzll(mask) : 0);
-}
 
 // The places of the waves' sorted lists (in LDS, `count` entries each) in the list of all of them: own place plus how many
 // of every other list come before.
@@ -201,6 +239,28 @@ struct Exponential {
     for (int i = 5; i >= 0; --i) p = fma(p, f, c[i]);
     return __builtin_ldexp(fma(p, f, 1.0), (int)n);
   }
+  // Four at once, the steps of one between those of the others: sums[j] += e^(x[j] - m).  PLAIN: no x is 700 or more below
+  // m, and |m| is so small that x / ln 2 - m / ln 2 is as good as (x - m) / ln 2.
+  template <bool PLAIN>
+  __device__ __forceinline__ void add(double (&sums)[4], f32x4 x, double m) const {
+    double f[4], p[4];
+    int n[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double t = PLAIN ? fma((double)x[j], 1.4426950408889634, m * -1.4426950408889634)
+                             : fmax(((double)x[j] - m) * 1.4426950408889634, -1100.0);
+      const double r = __builtin_rint(t);
+      f[j] = t - r;
+      n[j] = (int)r;
+      p[j] = fma(c[7], f[j], c[6]);
+    }
+#pragma unroll
+    for (int i = 5; i >= 0; --i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = fma(p[j], f[j], c[i]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[j] += __builtin_ldexp(fma(p[j], f[j], 1.0), n[j]);
+  }
 };
 
 // The 16 logits of a lane in the tile at `at`: pieces of 4 side by side, -inf past the row's end.
@@ -227,7 +287,8 @@ struct BeamParts {
 };
 
 // Block (part, row): `tiles` tiles to a wave.
-__global__ __launch_bounds__(BEAM_THREADS) void beam_rows_kernel(const float* __restrict__ logits, int64_t row_stride, int V,
+// (four workgroups to a compute unit, as many as the launch has for each)
+__global__ __launch_bounds__(BEAM_THREADS, 4) void beam_rows_kernel(const float* __restrict__ logits, int64_t row_stride, int V,
                                                                  int count, int parts, int tiles, BeamParts out) {
   __shared__ float xs[BEAM_WAVES * BEAM_MAX_COUNT];
   __shared__ int is[BEAM_WAVES * BEAM_MAX_COUNT];
@@ -242,7 +303,7 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_rows_kernel(const float* __
   const Exponential exp_of;
   Best<float> best(count, wait_x[wave], wait_i[wave]);
   float m = -INFINITY;
-  double s = 0.0;
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
   // The part's tiles go round the waves.  Which lane adds up a logit follows from its index alone: equal rows have equal
   // sums wherever they lie.
   const int64_t first = ((int64_t)part * tiles * BEAM_WAVES + wave) * BEAM_TILE;
@@ -254,60 +315,65 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_rows_kernel(const float* __
     if (at >= V) break;
     f32x4 x[4];
     float top = -INFINITY;
-    bool nan = false;
+    float tops[4];                         // of a lane's pieces
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        x[j][c] = next[j][c];
-        nan |= x[j][c] != x[j][c];
-      }
-    if (__ballot(nan)) {                 // (counts as -inf)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) x[j][c] = x[j][c] == x[j][c] ? x[j][c] : -INFINITY;
+    for (int j = 0; j < 4; ++j) {
+      x[j] = next[j];
+      tops[j] = fmaxf(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])), -INFINITY);   // (of a NaN and another value the other)
+      top = fmaxf(top, tops[j]);
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) top = fmaxf(top, x[j][c]);
     if (t + 1 < tiles && at + step < V) load_tile(row, at + step, V, lane, next);
-    const float tile_top = wave_top(top);
+    const float tile_top = wave_top(top, lane);
     if (tile_top > m) {
-      s *= exp_of((double)m - (double)tile_top);
+      const double less = exp_of((double)m - (double)tile_top);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] *= less;
       m = tile_top;
     }
-    if (m == INFINITY) {                 // (only such logits have a share)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s += x[j][c] == INFINITY ? 1.0 : 0.0;
-    } else if (m > -INFINITY) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s += exp_of((double)x[j][c] - (double)m);
-    }
-    // the candidates: of the first tile those that reach what `count` lanes reach, then those that come before the last
-    // of the list
-    const float bar = t == 0 ? reached_by(top, count) : best.last_x;
+    // (mask values, infinities, NaN, far outliers)
+    bool odd = !(fabsf(m) < 1e4f);
+    const float low = m - 700.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (__ballot(x[j][c] >= bar) == 0) continue;
-        const int e = (int)at + (j * MI_WAVE + lane) * 4 + c;
-        best.take(x[j][c], e, (e < V) & (x[j][c] >= bar), lane);
+      for (int c = 0; c < 4; ++c) odd |= !(x[j][c] >= low);
+    if (__ballot(odd) == 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) exp_of.add<true>(sum, x[j], (double)m);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          x[j][c] = x[j][c] == x[j][c] ? x[j][c] : -INFINITY;         // a NaN counts as -inf
+          if (m == INFINITY) sum[c] += x[j][c] == INFINITY ? 1.0 : 0.0;         // (only such logits have a share)
+        }
+      if (m > -INFINITY && m < INFINITY) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) exp_of.add<false>(sum, x[j], (double)m);
       }
+    }
+    // the candidates
+    const float bar = t == 0 ? reached_by(top, count, lane) : best.last_x;
+    if (tile_top >= bar) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (__ballot(tops[j] >= bar) == 0) continue;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (__ballot(x[j][c] >= bar) == 0) continue;
+          const int e = (int)at + (j * MI_WAVE + lane) * 4 + c;
+          best.take(x[j][c], e, (e < V) & (x[j][c] >= bar), lane);
+        }
+      }
+    }
     best.join(lane, t == 0 || t + 1 == tiles || at + step >= V);
   }
   if (lane < count) {
     xs[wave * count + lane] = best.x;
     is[wave * count + lane] = best.i;
   }
-#pragma unroll
-  for (int o = MI_WAVE / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, MI_WAVE);
+  const double s = sum_of_lanes((sum[0] + sum[1]) + (sum[2] + sum[3]), lane);
   if (lane == 0) {
     maxima[wave] = m;
     sums[wave] = s;
@@ -324,11 +390,11 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_rows_kernel(const float* __
   if (threadIdx.x == 0) {
     float all = maxima[0];
     for (int w = 1; w < BEAM_WAVES; ++w) all = fmaxf(all, maxima[w]);
-    double sum = 0.0;
+    double total = 0.0;
     for (int w = 0; w < BEAM_WAVES; ++w)
-      sum += maxima[w] == all ? sums[w] : sums[w] * exp_of((double)maxima[w] - (double)all);
+      total += maxima[w] == all ? sums[w] : sums[w] * exp_of((double)maxima[w] - (double)all);
     out.max[to] = all;
-    out.sum[to] = sum;
+    out.sum[to] = total;
   }
 }
 
@@ -350,18 +416,24 @@ __global__ __launch_bounds__(WAVES * MI_WAVE) void beam_pick_kernel(const float*
   const Exponential exp_of;
   if (threadIdx.x == 0) special = 0;
   __syncthreads();
-  for (int b = wave; b < beams; b += WAVES) {
+  // 16 lanes to a row: what its parts say, all rows of a wave's lanes at once
+  for (int b0 = 0; b0 < beams; b0 += WAVES * 4) {
+    const int b = b0 + wave * 4 + lane / 16, l = lane & 15;
     float m = -INFINITY;
-    for (int p = lane; p < parts; p += MI_WAVE) m = fmaxf(m, in.max[(r0 + b) * parts + p]);
-    m = wave_max(m);
-    double s = 0.0;
-    for (int p = lane; p < parts; p += MI_WAVE) {
-      const float pm = in.max[(r0 + b) * parts + p];
-      s += pm == m ? in.sum[(r0 + b) * parts + p] : in.sum[(r0 + b) * parts + p] * exp_of((double)pm - (double)m);
-    }
+    if (b < beams)
+      for (int p = l; p < parts; p += 16) m = fmaxf(m, in.max[(r0 + b) * parts + p]);
 #pragma unroll
-    for (int o = MI_WAVE / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, MI_WAVE);
-    if (lane == 0) {
+    for (int step = 1; step < 16; step <<= 1) m = fmaxf(m, xor_lane(m, step, lane));
+    double s = 0.0;
+    if (b < beams)
+      for (int p = l; p < parts; p += 16) {
+        const float pm = in.max[(r0 + b) * parts + p];
+        const double ps = in.sum[(r0 + b) * parts + p];
+        s += pm == m ? ps : ps * exp_of((double)pm - (double)m);
+      }
+#pragma unroll
+    for (int step = 1; step < 16; step <<= 1) s += xor_lane(s, step, lane);
+    if (b < beams && l == 0) {
       const float start = scores[r0 + b];
       const bool dead = !(fabsf(start) < INFINITY) || m == -INFINITY;
       row_max[b] = m;
