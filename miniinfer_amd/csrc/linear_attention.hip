@@ -14,9 +14,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 #define LA_MAX_D 256
 
-__device__ __forceinline__ float decay_power(float log_decay, int n) {   // a^n; a^0 = 1 for a decay of zero too
-  return n == 0 ? 1.f : (float)exp((double)log_decay * n);
-}
+// a^n; a^0 = 1 for a decay of zero too.  (The product's rounding puts an error of |n log a| 2^-24 on the power, at most
+// 0.4 * 2^-24 of the weight 1 for a decay.)
+__device__ __forceinline__ float decay_power(float log_decay, int n) { return n == 0 ? 1.f : expf(log_decay * n); }
 
 // ---------------------------------------------------------------- single tokens
 //
@@ -171,7 +171,7 @@ MI_EXPORT int mi_linear_attention_step(LA_ARGS, hipStream_t stream) {
 
 // ---------------------------------------------------------------- prompts: chunks of C tokens on the matrix cores
 //
-// With S the state before a chunk, i and j tokens of it, n how many it has (the rest of its C rows are zeros):
+// With S the state before a chunk, i and j tokens of it, n how many it has (the rest of its C rows weigh nothing):
 //
 //   O[i]  = scale * ( a^(i+1) q_i S  +  sum_{j <= i} a^(i-j) (q_i . k_j) v_j )
 //   S'    = a^n S + sum_j a^(n-1-j) k_j v_j^T
@@ -185,11 +185,21 @@ MI_EXPORT int mi_linear_attention_step(LA_ARGS, hipStream_t stream) {
 //   O^T += V^T P^T     V^T by the LDS's transposing reads
 //   S  += K^T (w V)    K^T likewise
 //
-// An operand of the matrix cores is 4 consecutive elements along the axis that is summed, from 16 rows and 4 groups of
-// lanes (a "half"): bfloat16 takes two halves to a product (16x16x32), 32-bit one half to four (16x16x4).
 // Roundings of the bfloat16 form: what is 32-bit (S, the weighted P and w V) is split into bfloat16 parts that are
 // multiplied one after the other into the same accumulators: two parts (what is left out is 2^-17 of a term) for what
 // ends in a bfloat16 output, three (2^-25) for the state, which is 32-bit whatever the inputs are.
+//
+// Operands: lane l of an operand has row l % 16 and, of 32 elements of the summed axis, with g = l / 16: in bfloat16
+// (16x16x32) the 8 from 8 g on, in 32 bits (eight products 16x16x4) the 4 from 4 g on and the 4 from 16 + 4 g on.  Its
+// first and last 4 are a "half".  An accumulator's lane has column l % 16 and rows 4 g .. 4 g + 3, so that two
+// accumulators are the two halves of an operand: for S, whose rows are given out accordingly (`dim_of`).
+//
+// Q, K and V go straight from memory to LDS (lane i's 16 bytes land at base + 16 i), in tiles of whole rows, two chunks of
+// K and V and the Q of three query heads at a time, with the waits written out by count.  The piece of 16 bytes that a
+// lane asks for is chosen such that piece p of row r lies at place p ^ swap(r): then the operands' reads, 16 pieces at a
+// time (lanes 0-3, 12-15 and 20-27, ...), and the transposing reads, 16 times 8 bytes of 4 rows, meet no bank twice
+// (with p ^ 2 (r mod 4), as good for the former alone, the LDS was busy twice as long, and 32,768 tokens of 32 heads on
+// 8 of 128 took 209 us instead of 198, without the kernels for segments).
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -197,12 +207,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
-#ifndef LA_C64
-#define LA_C64 64
-#endif
-#ifndef LA_PBUF64
-#define LA_PBUF64 2
-#endif
 #define LA_LDS(T) __attribute__((address_space(3))) T
 
 template <typename T>
@@ -258,41 +262,124 @@ struct Split<float, PARTS> {
   static constexpr int parts = 1;
 };
 
-// Tiles in LDS are rows of tokens.  The two halves that a lane takes to a bfloat16 product, columns 4 g .. and
-// 16 + 4 g .. of every 32, lie side by side (column 16 x + 4 g + i of a block at place 8 g + 4 x + i), so that an
-// operand is one 16-byte read; 32-bit columns keep their order.  Rows are padded by 32 bytes: an operand read, which
-// takes 16 bytes to a lane from 16 rows and 4 neighbouring pieces, is served 4 rows x 2 pieces at a time, and these then
-// lie in different banks.
+// A tile of whole rows in LDS: piece p of row r lies at place p ^ swap(r) of it.
 template <typename T, int COLS>
 struct Tile {
-  static constexpr int stride = COLS * (int)sizeof(T) + 32;
-  // of the 4 columns from col on (a multiple of 4)
-  static __device__ __forceinline__ int at(int row, int col) {
-    if (sizeof(T) == 2) return row * stride + (col & ~31) * 2 + (col & 12) * 4 + (col & 16) / 2;
-    return row * stride + col * 4;
+  static constexpr int stride = COLS * (int)sizeof(T);
+  static constexpr int pieces = stride / 16;
+  static constexpr int block = stride < 256 ? stride : 256;      // of a row; swaps stay inside
+  static __device__ __forceinline__ int swap(int r) {
+    if (sizeof(T) == 4 && stride >= 256) return 4 * (r >> 2 & 3) ^ (r & 3);
+    return (r >> 2 & 1) * 2 ^ (stride >= 256 ? (r & 3) * 4 : stride >= 128 ? (r >> 1 & 1) * 4 : 0);
   }
-  static constexpr int bytes(int rows) { return rows * stride; }
+  static __device__ __forceinline__ int at(int row, int col) {
+    const int byte = col * (int)sizeof(T);
+    return row * stride + (((byte >> 4) ^ swap(row)) << 4) + (byte & 15);
+  }
+  // from a place in the first 64 bytes of a row to that in 64 bytes number x
+  static __device__ __forceinline__ int on(int place, int x) { return (place ^ (64 * x) % block) + 64 * x / block * block; }
 };
 
-// The halves of columns col .. col + 31 of the lane's row; `p`: where Tile::at puts (row, 4 g).
-__device__ __forceinline__ s16x8 halves_at(const char* p, int col, bf16*) { return *reinterpret_cast<const s16x8*>(p + col * 2); }
-__device__ __forceinline__ f32x8 halves_at(const char* p, int col, float*) {
-  return join(*reinterpret_cast<const f32x4*>(p + col * 4), *reinterpret_cast<const f32x4*>(p + col * 4 + 64));
+// Where a lane finds its pieces of operands of 16 rows in a tile
+template <typename T, int COLS>
+struct OperandAt {
+  int first;
+  __device__ __forceinline__ explicit OperandAt(int lane) : first(Tile<T, COLS>::at(lane & 15, lane / 16 * (16 / (int)sizeof(T)))) {}
+  // 16 rows from `row0` on (a multiple of 16), 64 bytes number x of each
+  __device__ __forceinline__ int operator()(int row0, int x) const { return row0 * Tile<T, COLS>::stride + Tile<T, COLS>::on(first, x); }
+};
+// An operand: 32 elements, number kt, of 16 rows.
+template <int COLS>
+__device__ __forceinline__ s16x8 operand(const char* tile, const OperandAt<bf16, COLS>& at, int row0, int kt) {
+  return *reinterpret_cast<const s16x8*>(tile + at(row0, kt));
+}
+template <int COLS>
+__device__ __forceinline__ f32x8 operand(const char* tile, const OperandAt<float, COLS>& at, int row0, int kt) {
+  return join(*reinterpret_cast<const f32x4*>(tile + at(row0, 2 * kt)), *reinterpret_cast<const f32x4*>(tile + at(row0, 2 * kt + 1)));
 }
 
-// Elements [row 4 g .. 4 g + 3] of column l % 16 of a 16 x 16 piece whose first element is at (row0, col0): the lane's
-// half along the rows.
+// Element i of half h of the lane's 32 elements number x, along a summed axis.
+template <typename T>
+__device__ __forceinline__ int summed(int x, int h, int g, int i) {
+  return sizeof(T) == 2 ? 32 * x + 8 * g + 4 * h + i : 32 * x + 16 * h + 4 * g + i;
+}
+// Row m of half h of the pair of accumulators number x, such that the pair is an operand.
+template <typename T>
+__device__ __forceinline__ int dim_of(int x, int h, int m) {
+  return sizeof(T) == 2 ? 32 * x + 8 * (m / 4) + 4 * h + m % 4 : 32 * x + 16 * h + m;
+}
+
+// Operands along the rows of a tile.  In bfloat16 by the LDS's transposing reads: of 16 lanes, lane 4 j + c brings 4
+// columns of row j and gets column l % 16 of the 4 rows.  (Not by the builtin, before which the compiler waits for
+// everything that is on its way to LDS.)
+template <typename T, int COLS>
+struct DownAt {
+  int v, k;                          // the first of 16 columns from col0 on; of those that are rows of accumulators
+  __device__ __forceinline__ DownAt(int lane, int col0) {
+    const int g = lane / 16, j = lane % 16 / 4, c = lane % 4;
+    if (sizeof(T) == 2) {
+      v = Tile<T, COLS>::at(8 * g + j, col0 + 4 * c);
+      k = Tile<T, COLS>::at(8 * g + j, dim_of<T>(0, 0, 4 * c));
+    } else {
+      v = Tile<T, COLS>::at(4 * g, col0 + lane % 16);
+      k = Tile<T, COLS>::at(4 * g, lane % 16);
+    }
+  }
+};
+__device__ __forceinline__ uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(LA_LDS(char)*)p; }
+
+// Rows 32 x .. 32 x + 31, 16 columns
 template <int COLS>
-__device__ __forceinline__ s16x4 half_down(const char* tile, int row0, int col0, int lane, bf16*) {
-  const char* p = tile + Tile<bf16, COLS>::at(row0 + lane / 16 * 4 + lane % 16 / 4, col0 + lane % 4 * 4);
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((LA_LDS(s16x4)*)(LA_LDS(char)*)p);
+__device__ __forceinline__ s16x8 columns_down(const char* tile, const DownAt<bf16, COLS>& at, int x) {
+  const uint32_t from = lds_address(tile) + 32 * x * Tile<bf16, COLS>::stride;
+  s16x4 lo, hi;                      // (rows 4 on are swapped by 2 pieces more)
+  asm volatile("ds_read_b64_tr_b16 %0, %2\n\t"
+               "ds_read_b64_tr_b16 %1, %3 offset:%4\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(lo), "=&v"(hi)
+               : "v"(from + at.v), "v"(from + (at.v ^ 32)), "n"(4 * Tile<bf16, COLS>::stride)
+               : "memory");
+  return join(lo, hi);
 }
 template <int COLS>
-__device__ __forceinline__ f32x4 half_down(const char* tile, int row0, int col0, int lane, float*) {
-  f32x4 r;
+__device__ __forceinline__ f32x8 columns_down(const char* tile, const DownAt<float, COLS>& at, int x) {
+  f32x8 r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const float*>(tile + (row0 + lane / 16 * 4 + i) * Tile<float, COLS>::stride + (col0 + lane % 16) * 4);
+  for (int i = 0; i < 8; ++i)        // (row 4 g + i: swapped by i more)
+    r[i] = *reinterpret_cast<const float*>(tile + (at.v ^ 16 * (i % 4)) + summed<float>(x, i / 4, 0, i % 4) * Tile<float, COLS>::stride);
   return r;
+}
+// Rows 32 x .. 32 x + 31 of the columns that are the rows of the accumulators (kt, 0), (kt, 1), (kt + 1, 0), (kt + 1, 1);
+// kt is even
+template <int COLS>
+__device__ __forceinline__ void dims_down(s16x8 (&r)[2][2], const char* tile, const DownAt<bf16, COLS>& at, int x, int kt) {
+  const uint32_t from = lds_address(tile) + 32 * x * Tile<bf16, COLS>::stride;
+  const uint32_t k0 = from + Tile<bf16, COLS>::on(at.k, kt), k1 = from + Tile<bf16, COLS>::on(at.k, kt + 1);
+  s16x4 p[8];
+  asm volatile("ds_read_b64_tr_b16 %0, %8\n\t"
+               "ds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
+               "ds_read_b64_tr_b16 %2, %8 offset:8\n\t"
+               "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+               "ds_read_b64_tr_b16 %4, %10\n\t"
+               "ds_read_b64_tr_b16 %5, %11 offset:%12\n\t"
+               "ds_read_b64_tr_b16 %6, %10 offset:8\n\t"
+               "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(p[0]), "=&v"(p[1]), "=&v"(p[2]), "=&v"(p[3]), "=&v"(p[4]), "=&v"(p[5]), "=&v"(p[6]), "=&v"(p[7])
+               : "v"(k0), "v"(k0 ^ 32), "v"(k1), "v"(k1 ^ 32), "n"(4 * Tile<bf16, COLS>::stride),
+                 "n"(4 * Tile<bf16, COLS>::stride + 8)
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i / 2][i % 2] = join(p[2 * i], p[2 * i + 1]);
+}
+template <int COLS>
+__device__ __forceinline__ void dims_down(f32x8 (&r)[2][2], const char* tile, const DownAt<float, COLS>& at, int x, int kt) {
+#pragma unroll
+  for (int y = 0; y < 4; ++y)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      r[y / 2][y % 2][i] = *reinterpret_cast<const float*>(tile + Tile<float, COLS>::on(at.k ^ 16 * (i % 4), 2 * kt + y) +
+                                                           summed<float>(x, i / 4, 0, i % 4) * Tile<float, COLS>::stride);
 }
 
 // 16 bytes from p on, element by element
@@ -304,69 +391,70 @@ __device__ __forceinline__ u32x4 piece_of_elements(const T* p) {
   return __builtin_bit_cast(u32x4, tmp);
 }
 
-// A thread's pieces (16 bytes) of a tile of C rows: rows r0, r0 + step, ... at column c0.
-template <typename T, int COLS, int C, int THREADS>
-struct Pieces {
-  static constexpr int to_row = COLS * (int)sizeof(T) / 16, step = THREADS / to_row, count = C / step;
-  static_assert(THREADS % to_row == 0 && C % step == 0, "whole rows to a round");
-  int r0, c0;
-  uint32_t offset;                   // of the first piece, in bytes, from the tile's first element in memory
-  int lds;
-  bool live;
-  u32x4 held[count];
-  __device__ __forceinline__ Pieces(int tid, int64_t stride, int columns) {
-    r0 = tid / to_row;
-    c0 = tid % to_row * (16 / (int)sizeof(T));
-    live = c0 < columns;
-    offset = (uint32_t)((r0 * stride + c0) * (int)sizeof(T));
-    lds = Tile<T, COLS>::at(r0, c0);
+// A wave's share of the way of a tile of C rows from memory to LDS: `count` requests of 1 KB.  Columns past the end are
+// never written (they are zeros from the start); rows past the last token are that token's again: the weights of such
+// tokens are zeros.  Not ALIGNED: the elements one by one through registers.
+template <typename T, int COLS, int C, int WAVES>
+struct Loader {
+  typedef Tile<T, COLS> Shape;
+  static constexpr int rows = MI_WAVE / Shape::pieces, count = C / rows / WAVES;
+  static_assert(MI_WAVE % Shape::pieces == 0 && C % (rows * WAVES) == 0, "whole rows to a request");
+  int row0, column[count];             // column: of the lane's piece; -1: past the end
+  uint32_t offset[count];              // bytes from the tile's first element
+  __device__ __forceinline__ Loader(int wave, int lane, int64_t stride, int columns) {
+    row0 = wave * count * rows + lane / Shape::pieces;
+#pragma unroll
+    for (int i = 0; i < count; ++i) {
+      const int row = row0 + i * rows;
+      column[i] = ((lane % Shape::pieces) ^ Shape::swap(row)) * (16 / (int)sizeof(T));
+      if (column[i] >= columns) column[i] = -1;
+      offset[i] = (uint32_t)((row * stride + column[i]) * (int)sizeof(T));
+    }
   }
-  // n rows from `from` on; the rest, and columns past the end, are zeros
   template <bool ALIGNED>
-  __device__ __forceinline__ void load(const T* from, int64_t stride, int n) {
+  __device__ __forceinline__ void load(const T* from, int64_t stride, int n, char* tile, int wave, int lane) const {
+    char* to = tile + wave * count * 1024;
     if (ALIGNED && n == C) {
 #pragma unroll
-      for (int i = 0; i < count; ++i) {
-        held[i] = u32x4{0, 0, 0, 0};
-        if (live) held[i] = *reinterpret_cast<const u32x4*>((const char*)(from + i * step * stride) + offset);
-      }
+      for (int i = 0; i < count; ++i)
+        if (column[i] >= 0) request((const char*)from + offset[i], to + i * 1024);
     } else {
 #pragma unroll
       for (int i = 0; i < count; ++i) {
-        held[i] = u32x4{0, 0, 0, 0};
-        if (live && r0 + i * step < n) {
-          const T* at = from + (r0 + i * step) * stride + c0;
-          held[i] = ALIGNED ? *reinterpret_cast<const u32x4*>(at) : piece_of_elements(at);
-        }
+        if (column[i] < 0) continue;
+        const T* at = from + min(row0 + i * rows, n - 1) * stride + column[i];
+        if (ALIGNED)
+          request(at, to + i * 1024);
+        else
+          *reinterpret_cast<u32x4*>(to + i * 1024 + lane * 16) = piece_of_elements(at);
       }
     }
   }
-  __device__ __forceinline__ void store(char* tile) const {
-#pragma unroll
-    for (int i = 0; i < count; ++i) {
-      char* at = tile + lds + i * step * Tile<T, COLS>::stride;
-      if (sizeof(T) == 2) {              // columns c0 .. c0 + 3 and the next 4
-        *reinterpret_cast<mi_u32x2*>(at) = mi_u32x2{held[i][0], held[i][1]};
-        *reinterpret_cast<mi_u32x2*>(at + 16) = mi_u32x2{held[i][2], held[i][3]};
-      } else {
-        *reinterpret_cast<u32x4*>(at) = held[i];
-      }
-    }
+  static __device__ __forceinline__ void request(const void* from, char* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (LA_LDS(void)*)to, 16, 0, 0);
   }
 };
 
-__device__ __forceinline__ bool all_finite(u32x4 x, bf16*) {
+// All but the last `N` requests to memory of the wave are done, and every wave's LDS accesses; the waves meet.
+template <int N>
+__device__ __forceinline__ void arrive() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ bool all_finite(s16x8 x) {
   bool ok = true;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) ok = ok && (x[i] & 0x7f80u) != 0x7f80u && (x[i] & 0x7f800000u) != 0x7f800000u;
+  for (int i = 0; i < 8; ++i) ok &= (x[i] & 0x7f80) != 0x7f80;
   return ok;
 }
-__device__ __forceinline__ bool all_finite(u32x4 x, float*) {
+__device__ __forceinline__ bool all_finite(f32x8 x) {
   bool ok = true;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) ok = ok && (x[i] & 0x7f800000u) != 0x7f800000u;
+  for (int i = 0; i < 8; ++i) ok &= fabsf(x[i]) < INFINITY;
   return ok;
 }
+__device__ __forceinline__ f32x4 half_of(s16x8 x, int h) { return h ? widen(__builtin_shufflevector(x, x, 4, 5, 6, 7)) : widen(__builtin_shufflevector(x, x, 0, 1, 2, 3)); }
+__device__ __forceinline__ f32x4 half_of(f32x8 x, int h) { return h ? __builtin_shufflevector(x, x, 4, 5, 6, 7) : __builtin_shufflevector(x, x, 0, 1, 2, 3); }
 
 struct LinearAttention {
   const void *q, *k, *v;
@@ -391,55 +479,64 @@ __device__ __forceinline__ int first_unit(const LinearAttention& a, int b) {
   return min(max(a.cu[b], 0), a.num_tokens) / a.segment + b;
 }
 
-template <typename T, int DP, int WAVES, int C, int PBUF>
+// QBUF, PBUF, KBUF: buffers of Q, of P and, for the segments' states, of K and V (2 otherwise).
+template <typename T, int DP, int WAVES, int C, int QBUF, int PBUF, int KBUF>
 struct ChunkShape {
   static constexpr int waves = WAVES, threads = 64 * WAVES;
   static constexpr int VS = 16 * waves;
-  static constexpr int kt = DP / 16, ct = C / 16;
-  static constexpr int q_bytes = (Tile<T, DP>::bytes(C) + 15) / 16 * 16;
-  static constexpr int v_bytes = (Tile<T, VS>::bytes(C) + 15) / 16 * 16;
-  static constexpr int part_bytes = (Tile<T, C>::bytes(C) + 15) / 16 * 16;
-  static constexpr int p_bytes = (sizeof(T) == 2 ? 2 : 1) * part_bytes;
-  static constexpr int lds(bool states) { return 2 * (q_bytes + v_bytes) + (states ? 0 : 2 * q_bytes + PBUF * p_bytes); }
+  static constexpr int parts = sizeof(T) == 2 ? 2 : 1;
+  static constexpr int q_bytes = C * Tile<T, DP>::stride, v_bytes = C * Tile<T, VS>::stride;
+  static constexpr int part_bytes = C * Tile<T, C>::stride, p_bytes = parts * part_bytes;
+  static constexpr int lds(bool states) {
+    return states ? KBUF * (q_bytes + v_bytes) : 2 * (q_bytes + v_bytes) + QBUF * q_bytes + PBUF * p_bytes;
+  }
 };
 
+// What bounds it (that workload, 198 us at 3.4 TB/s): the matrix cores are busy for 30% of the time, the vector ALUs and the
+// LDS for about as long, memory for half of it.  With 8 waves on a compute unit, all that the registers (256) and the LDS
+// (144 KB) allow, the waits between a head's products are not covered: without loads and stores it takes 142 us, without
+// stores 25 less, without any one of the products 0 to 17 less.  Smaller chunks (32 tokens) with twice the workgroups are
+// slower with heads of 128 (256 us for the whole call, 234) and faster with heads up to 64 (8,192 tokens, 32 heads:
+// 76 us, 114).
+//
 // STATES: only what a segment adds to its request's state (from zero), left in `work`; the last segment's is not needed.
 // ALIGNED: rows of q, k and v start at multiples of 16 bytes, of out at multiples of 4 elements, and a chunk of a tensor
 // spans less than 2^31 bytes.
-template <typename T, int DP, int WAVES, int C, int PBUF, bool STATES, bool ALIGNED, int PER_SIMD>
+template <typename T, int DP, int WAVES, int C, int QBUF, int PBUF, int KBUF, bool STATES, bool ALIGNED, int PER_SIMD>
 __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAttention a) {
-  typedef ChunkShape<T, DP, WAVES, C, PBUF> Shape;
+  typedef ChunkShape<T, DP, WAVES, C, QBUF, PBUF, KBUF> Shape;
   typedef typename Half<T>::type half;
   typedef typename Half<T>::pair pair;
-  constexpr int PARTS = Split<T, 2>::parts;
-  typedef Tile<T, DP> QTile;
-  typedef Tile<T, Shape::VS> VTile;
-  typedef Tile<T, C> PTile;
-  constexpr int KT = Shape::kt, CT = Shape::ct, VS = Shape::VS;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int PARTS = Shape::parts, KX = DP / 32, KB = KX < 4 ? KX : 4, CX = C / 32, CT = C / 16, VS = Shape::VS;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
   __shared__ float power[C + 1];     // a^i
   __shared__ float left[2 * C];      // a^(C-1-i), zeros from C on
-  __shared__ int found, not_finite[2];
+  __shared__ int found;
   char* const k_lds = lds;
-  char* const v_lds = k_lds + 2 * Shape::q_bytes;
-  char* const q_lds = v_lds + 2 * Shape::v_bytes;
-  char* const p_lds = q_lds + 2 * Shape::q_bytes;
+  char* const v_lds = k_lds + (STATES ? KBUF : 2) * Shape::q_bytes;
+  char* const q_lds = v_lds + (STATES ? KBUF : 2) * Shape::v_bytes;
+  char* const p_lds = q_lds + QBUF * Shape::q_bytes;
 
-  const int tid = threadIdx.x, lane = tid & (MI_WAVE - 1), wave = tid / MI_WAVE, l16 = lane & 15, g4 = lane / 16 * 4;
+  const int tid = threadIdx.x, lane = tid & (MI_WAVE - 1), l16 = lane & 15, g = lane / 16, g4 = 4 * g;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / MI_WAVE);
   const int slices = (a.d + VS - 1) / VS;
   const int h = blockIdx.x % a.nkv, slice = blockIdx.x / a.nkv % slices, unit = blockIdx.x / (a.nkv * slices);
   const int d = a.d;
 
   int b = unit, lo, hi, segment = 0, segments = 1;
   if (a.segment) {
-    if (tid == 0) found = 0;
-    __syncthreads();
-    int n = 0;
-    for (int i = tid; i < a.num_requests; i += Shape::threads) n += first_unit(a, i) <= unit;
-    if (n) atomicAdd(&found, n);
-    __syncthreads();
-    b = found - 1;
-    if (b < 0) return;
+    if (a.num_requests == 1) {
+      b = 0;
+    } else {
+      if (tid == 0) found = 0;
+      __syncthreads();
+      int n = 0;
+      for (int i = tid; i < a.num_requests; i += Shape::threads) n += first_unit(a, i) <= unit;
+      if (n) atomicAdd(&found, n);
+      __syncthreads();
+      b = found - 1;
+      if (b < 0) return;
+    }
     bounds_of(a, b, lo, hi);
     segment = unit - first_unit(a, b);
     segments = (hi - lo + a.segment - 1) / a.segment;
@@ -453,6 +550,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
   if (lo >= hi) return;
 
   const int n0 = slice * VS + wave * 16;                 // first column of the wave
+  const bool columns = n0 < d;                           // whether it has any: else it helps with loads and P only
   const int row = a.rows[b];
   T* const out = (T*)a.out;
   if (row < 0 || row >= a.num_rows) {                    // no such state: rows of NaN
@@ -463,100 +561,151 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
             out[(int64_t)t * a.out_stride + (int64_t)(h * a.rep + i / VS) * d + slice * VS + i % VS] = from_float<T>(NAN);
     return;
   }
-  for (int i = tid; i <= C; i += Shape::threads) power[i] = decay_power(a.log_decay[h], i);
-  for (int i = tid; i < 2 * C; i += Shape::threads) left[i] = i < C ? decay_power(a.log_decay[h], C - 1 - i) : 0.f;
-  if (tid < 2) not_finite[tid] = 0;
+  if (tid <= C) {
+    const float p = decay_power(a.log_decay[h], tid);
+    power[tid] = p;
+    if (tid < C) left[C - 1 - tid] = p;
+  }
+  for (int i = C + tid; i < 2 * C; i += Shape::threads) left[i] = 0.f;
+  if (d < DP || d < (slice + 1) * VS)                    // columns past the end
+    for (int i = tid; i < Shape::lds(STATES) / 16; i += Shape::threads) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
   __syncthreads();
 
-  // the wave's columns of the state, accumulator t: rows 16 t + g4 + i, column n0 + l16
-  f32x4 s[KT];
+  // the wave's columns of the state, accumulators (x, y): row dim_of(x, y, g4 + i), column n0 + l16
+  f32x4 s[KX][2];
   float* const s_row = a.state + (int64_t)row * a.state_stride + (int64_t)h * d * d;
   float* const s_work = a.segment ? a.work + ((int64_t)unit * a.nkv + h) * d * d : nullptr;
   const float* const s_from = segments > 1 ? s_work : row == a.idle_row ? nullptr : s_row;
-#pragma unroll
-  for (int t = 0; t < KT; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 16 * t + g4 + i, c = n0 + l16;
-      s[t][i] = !STATES && s_from && r < d && c < d ? s_from[(int64_t)r * d + c] : 0.f;
-    }
 
   const T* const kp = (const T*)a.k + (int64_t)h * d;
   const T* const vp = (const T*)a.v + (int64_t)h * d + slice * VS;
   const T* const qp = (const T*)a.q + (int64_t)h * a.rep * d;
+  const Loader<T, DP, C, WAVES> k_way(wave, lane, a.k_stride, d), q_way(wave, lane, a.q_stride, d);
+  const Loader<T, VS, C, WAVES> v_way(wave, lane, a.v_stride, d - slice * VS);
+  constexpr int QN = ALIGNED ? q_way.count : 0, KVN = ALIGNED ? k_way.count + v_way.count : 0;     // requests of a wave
+  auto load_kv = [&](int t, int n, int buf) {
+    k_way.template load<ALIGNED>(kp + t * a.k_stride, a.k_stride, n, k_lds + buf * Shape::q_bytes, wave, lane);
+    v_way.template load<ALIGNED>(vp + t * a.v_stride, a.v_stride, n, v_lds + buf * Shape::v_bytes, wave, lane);
+  };
+  auto load_state = [&]() {
+#pragma unroll
+    for (int x = 0; x < KX; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = dim_of<T>(x, y, g4 + i), c = n0 + l16;
+          s[x][y][i] = 0.f;
+          if (!STATES && s_from && r < d && c < d) s[x][y][i] = s_from[(int64_t)r * d + c];
+        }
+  };
 
-  Pieces<T, DP, C, Shape::threads> kr(tid, a.k_stride, d), qr(tid, a.q_stride, d);
-  Pieces<T, VS, C, Shape::threads> vr(tid, a.v_stride, d - slice * VS);
-  auto load_k = [&](int t, int n) {
-    kr.template load<ALIGNED>(kp + t * a.k_stride, a.k_stride, n);
-    vr.template load<ALIGNED>(vp + t * a.v_stride, a.v_stride, n);
-  };
-  auto load_q = [&](int t, int n, int g) { qr.template load<ALIGNED>(qp + t * a.q_stride + g * d, a.q_stride, n); };
-  auto store_k = [&](int buf) -> bool {      // whether a value is not finite
-    kr.store(k_lds + buf * Shape::q_bytes);
-    vr.store(v_lds + buf * Shape::v_bytes);
-    bool ok = true;
+  const DownAt<T, DP> k_down(lane, 0);
+  const DownAt<T, VS> v_down(lane, wave * 16);
+  pair vt[CX];                       // V^T of the chunk: the wave's 16 columns
+  auto read_v = [&](int buf, int n) {
 #pragma unroll
-    for (int i = 0; i < vr.count; ++i) ok = ok && all_finite(vr.held[i], (T*)nullptr);
-    return !ok;
-  };
-  half vt[CT];                       // V^T of the chunk: the wave's 16 columns, tokens 16 jt + g4 + i
-  T* const typed = nullptr;          // (picks an overload)
-  auto read_v = [&](int buf) {
+    for (int x = 0; x < CX; ++x) {
+      vt[x] = columns_down(v_lds + buf * Shape::v_bytes, v_down, x);
+      if (n < C) {                   // (a weight of zero times what is not finite is not zero)
 #pragma unroll
-    for (int jt = 0; jt < CT; ++jt) vt[jt] = half_down<VS>(v_lds + buf * Shape::v_bytes, 16 * jt, wave * 16, lane, typed);
+        for (int i = 0; i < 8; ++i)
+          if (summed<T>(x, i / 4, g, i % 4) >= n) vt[x][i] = 0;
+      }
+    }
   };
   auto update = [&](int buf, int n) {        // the state after a chunk of n tokens
     const char* const kb = k_lds + buf * Shape::q_bytes;
     const float an = power[n];
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) s[kt] *= an;
+    for (int x = 0; x < KX; ++x)
 #pragma unroll
-    for (int jt = 0; jt < CT; jt += 2) {
-      pair kp[KT];
+      for (int y = 0; y < 2; ++y) s[x][y] *= an;
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-        kp[kt] = join(half_down<DP>(kb, 16 * jt, 16 * kt, lane, typed), half_down<DP>(kb, 16 * jt + 16, 16 * kt, lane, typed));
-      f32x4 w0, w1;                  // a^(n-1-j)
+    for (int j = 0; j < CX; ++j) {
+      f32x4 w[2];                    // a^(n-1-token)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w0[i] = left[C - n + 16 * jt + g4 + i];
-        w1[i] = left[C - n + 16 * jt + 16 + g4 + i];
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[y][i] = left[C - n + summed<T>(j, y, g, i)];
+      const Split<T, 3> v0(half_of(vt[j], 0) * w[0]), v1(half_of(vt[j], 1) * w[1]);
+#pragma unroll
+      for (int x0 = 0; x0 < KX; x0 += 2) {
+        pair kd[2][2];
+        dims_down(kd, kb, k_down, j, x0);
+#pragma unroll
+        for (int z = 0; z < Split<T, 3>::parts; ++z)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) mma(s[x0 + x][y], kd[x][y], join(v0.part[z], v1.part[z]));
       }
-      __builtin_amdgcn_sched_barrier(0);     // (the reads are on their way together)
-      const Split<T, 3> v0(widen(vt[jt]) * w0), v1(widen(vt[jt + 1]) * w1);
-#pragma unroll
-      for (int z = 0; z < Split<T, 3>::parts; ++z)
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) mma(s[kt], kp[kt], join(v0.part[z], v1.part[z]));
     }
   };
 
-  // The chunk at hand has the n tokens from t on.  Tiles are double-buffered: while one chunk (K, V) or query head (Q) is
-  // worked on, the next one's pieces are on their way in registers; they are stored to the other buffer before the one
-  // barrier of each step, and the loads after them are issued at once.
+  // The chunk at hand has the n tokens from t on.
   int t = lo, n = min(C, hi - lo), kv = 0;
   if constexpr (STATES) {
-    load_k(t, n);
-    store_k(0);
-    if (t + n < hi) load_k(t + n, min(C, hi - t - n));
-    __syncthreads();
+    // chunks go round KBUF buffers: KBUF - 1 are on their way while one is worked on
+    load_state();
+    int next = lo, slot = 0;
+    auto fetch = [&]() {
+      if (next >= hi) return false;
+      load_kv(next, min(C, hi - next), slot);
+      next += C;
+      slot = slot + 1 == KBUF ? 0 : slot + 1;
+      return true;
+    };
+#pragma unroll
+    for (int i = 0; i + 1 < KBUF; ++i) fetch();
+    if (next >= hi) arrive<0>();               // (at most KBUF - 1 chunks: all have to be here in the end)
+    else arrive<(KBUF - 2) * KVN>();
     for (;;) {
-      read_v(kv);
-      update(kv, n);
+      const bool more = fetch();
+      if (columns) {
+        read_v(kv, n);
+        update(kv, n);
+      }
       t += n;
       if (t >= hi) break;
       n = min(C, hi - t);
-      kv ^= 1;
-      store_k(kv);
-      if (t + n < hi) load_k(t + n, min(C, hi - t - n));
-      __syncthreads();
+      kv = kv + 1 == KBUF ? 0 : kv + 1;
+      if (more) arrive<(KBUF - 2) * KVN>();
+      else arrive<0>();
     }
   } else {
     const uint32_t out_offset = (uint32_t)((l16 * a.out_stride + n0 + g4) * (int)sizeof(T));
-    const int lane_q = QTile::at(l16, g4), lane_p = PTile::at(l16, g4);
+    const OperandAt<T, DP> q_at(lane);
+    const OperandAt<T, C> p_at(lane);
+    // the query head whose Q is fetched next: head fg of tokens ft .. ft + fn - 1; Q goes round QBUF buffers
+    int ft = t, fn = n, fg = 0, slot = 0;
+    auto fetch_q = [&]() {
+      if (ft >= hi) return false;
+      q_way.template load<ALIGNED>(qp + ft * a.q_stride + fg * d, a.q_stride, fn, q_lds + slot * Shape::q_bytes, wave, lane);
+      slot = slot + 1 == QBUF ? 0 : slot + 1;
+      if (++fg == a.rep) {
+        fg = 0;
+        ft += fn;
+        fn = min(C, hi - ft);
+      }
+      return true;
+    };
+    // K and V: the chunk after next is asked for at the end of a chunk
+    auto fetch_kv = [&](int from, int buf) {
+      if (from >= hi) return false;
+      load_kv(from, min(C, hi - from), buf);
+      return true;
+    };
+    load_kv(t, n, 0);
+    fetch_q();
+    load_state();
+    const bool next_kv = fetch_kv(t + C, 1);
+    bool q_new = false, kv_new = false;        // whether what was asked for last holds a Q, and K and V;
+    bool stored = false;                       // and whether CT stores to out came after it
+#pragma unroll
+    for (int i = 1; i < QBUF; ++i) q_new = fetch_q();
     // the weights a^(i-j) of the P that the wave makes, and a^(i+1) of its tokens, both with the scale
-    constexpr int PW = (CT * CT / 2 + WAVES - 1) / WAVES;
+    constexpr int PW = (CT * CX + WAVES - 1) / WAVES;
     int reach[PW];                   // i - j of a lane's first element: those of the next ones are less
     f32x4 weight[PW][2];
     float reached[CT];
@@ -574,78 +723,57 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     for (int ib = 0; ib < CT; ++ib) reached[ib] = power[16 * ib + l16 + 1] * a.scale;
     // the state's parts, held for all query heads of a chunk where there are registers for them
     constexpr bool HELD = DP <= 128;
-    pair sp[HELD ? KT / 2 : 1][PARTS];
-    // Tokens before `careful` go one to a chunk: a masked weight of zero times a value that is not finite would reach
-    // the tokens before it.
-    int careful = lo;
-    auto tokens_at = [&](int t) { return t < careful ? 1 : min(C, hi - t); };
-    // the query head whose Q is on its way: of tokens nt .. nt + nn - 1
-    int nt = t, nn = n, ng = 0;
-    auto fetch_next_q = [&]() {
-      if (++ng == a.rep) {
-        ng = 0;
-        nt += nn;
-        nn = tokens_at(nt);
-      }
-      if (nt < hi) load_q(nt, nn, ng);
-    };
-    load_k(t, n);
-    load_q(t, n, 0);
-    if (store_k(0)) not_finite[0] = 1;
-    qr.store(q_lds);
-    fetch_next_q();
-    if (t + n < hi) load_k(t + n, tokens_at(t + n));
-    __syncthreads();
-    int g = 0, qb = 0, pb = 0;
+    pair sp[HELD ? KX : 1][PARTS];
+    bool odd = false;                // whether one of the wave's values is not finite
+    if (next_kv && q_new) arrive<KVN + (QBUF - 1) * QN>();
+    else arrive<0>();
+    // (the state is here: else the compiler would wait for it, and for all that came after it, in every turn)
+#pragma unroll
+    for (int x = 0; x < KX; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) asm volatile("" : "+v"(s[x][y]));
+    int head = 0, qb = 0, pb = 0;
     for (;;) {
-      if (g == 0) {
-        if (not_finite[kv]) {          // the first of this chunk's tokens alone
-          __syncthreads();
-          if (tid == 0) not_finite[kv] = 0;
-          if (n > 1) {
-            careful = t + n;
-            n = 1;
-            load_k(t, n);
-            load_q(t, n, 0);
-            store_k(kv);
-            qr.store(q_lds + qb * Shape::q_bytes);
-            nt = t, nn = n, ng = 0;
-            fetch_next_q();
-            if (t + n < hi) load_k(t + n, tokens_at(t + n));
-          }
-          __syncthreads();
-        }
-        read_v(kv);
+      const bool last = head + 1 == a.rep;
+      if (head == 0 && columns) {
+        read_v(kv, n);
+        odd = false;
+#pragma unroll
+        for (int x = 0; x < CX; ++x) odd |= !all_finite(vt[x]);
+        odd = __ballot(odd) != 0;
         if (HELD) {
 #pragma unroll
-          for (int kt = 0; kt < KT / 2; ++kt) {
-            const Split<T, 2> s0(s[2 * kt]), s1(s[2 * kt + 1]);
+          for (int x = 0; x < KX; ++x) {
+            const Split<T, 2> s0(s[x][0]), s1(s[x][1]);
 #pragma unroll
-            for (int z = 0; z < PARTS; ++z) sp[kt][z] = join(s0.part[z], s1.part[z]);
+            for (int z = 0; z < PARTS; ++z) sp[x][z] = join(s0.part[z], s1.part[z]);
           }
         }
       }
-      const char* const qt = q_lds + qb * Shape::q_bytes + lane_q;
-      const char* const kt_lds = k_lds + kv * Shape::q_bytes + lane_q;
-      char* const pt = p_lds + pb * Shape::p_bytes + lane_p;
+      const char* const qt = q_lds + qb * Shape::q_bytes;
+      const char* const kt = k_lds + kv * Shape::q_bytes;
+      char* const pt = p_lds + pb * Shape::p_bytes;
       // ---- P^T: to a wave 16 queries and 32 tokens, or that again for the next waves' worth of them
 #pragma unroll
       for (int y = 0; y < PW; ++y) {
-        const int x = wave + y * WAVES, ib = x % CT, jt = x / CT * 2;
-        if (x >= CT * CT / 2 || jt > ib) continue;             // (no product below reads these)
-        pair qf[KT / 2], k0[KT / 2], k1[KT / 2];
-#pragma unroll
-        for (int kt = 0; kt < KT / 2; ++kt) {
-          qf[kt] = halves_at(qt + 16 * ib * QTile::stride, 32 * kt, typed);
-          k0[kt] = halves_at(kt_lds + 16 * jt * QTile::stride, 32 * kt, typed);
-          k1[kt] = halves_at(kt_lds + (16 * jt + 16) * QTile::stride, 32 * kt, typed);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        const int x = wave + y * WAVES, ib = x % CT, jx = x / CT;
+        if (x >= CT * CX || 2 * jx > ib) continue;             // (no product below reads these)
         f32x4 p0 = {0.f, 0.f, 0.f, 0.f}, p1 = p0;
 #pragma unroll
-        for (int kt = 0; kt < KT / 2; ++kt) {
-          mma(p0, k0[kt], qf[kt]);
-          mma(p1, k1[kt], qf[kt]);
+        for (int x0 = 0; x0 < KX; x0 += KB) {
+          pair qf[KB], k0[KB], k1[KB];
+#pragma unroll
+          for (int kx = 0; kx < KB; ++kx) {
+            qf[kx] = operand(qt, q_at, 16 * ib, x0 + kx);
+            k0[kx] = operand(kt, q_at, 32 * jx, x0 + kx);
+            k1[kx] = operand(kt, q_at, 32 * jx + 16, x0 + kx);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int kx = 0; kx < KB; ++kx) {
+            mma(p0, k0[kx], qf[kx]);
+            mma(p1, k1[kx], qf[kx]);
+          }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -655,64 +783,98 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
         const Split<T, 2> s0(p0), s1(p1);
 #pragma unroll
         for (int z = 0; z < PARTS; ++z) {
-          char* at = pt + z * Shape::part_bytes + 16 * ib * PTile::stride;
-          *reinterpret_cast<half*>(at + PTile::at(0, 16 * jt)) = s0.part[z];
-          *reinterpret_cast<half*>(at + PTile::at(0, 16 * jt + 16)) = s1.part[z];
+          char* at = pt + z * Shape::part_bytes;
+          *reinterpret_cast<half*>(at + Tile<T, C>::at(16 * ib + l16, 32 * jx + g4)) = s0.part[z];
+          *reinterpret_cast<half*>(at + Tile<T, C>::at(16 * ib + l16, 32 * jx + 16 + g4)) = s1.part[z];
         }
       }
       // ---- what the state gives
       f32x4 o[CT];
 #pragma unroll
       for (int ib = 0; ib < CT; ++ib) o[ib] = f32x4{0.f, 0.f, 0.f, 0.f};
-      pair qf[2][CT];
+      if (columns) {
+        pair qf[2][CT];
 #pragma unroll
-      for (int ib = 0; ib < CT; ++ib) qf[0][ib] = halves_at(qt + 16 * ib * QTile::stride, 0, typed);
+        for (int ib = 0; ib < CT; ++ib) qf[0][ib] = operand(qt, q_at, 16 * ib, 0);
 #pragma unroll
-      for (int kt = 0; kt < KT / 2; ++kt) {
-        if (kt + 1 < KT / 2) {
+        for (int x = 0; x < KX; ++x) {
+          if (x + 1 < KX) {
 #pragma unroll
-          for (int ib = 0; ib < CT; ++ib) qf[(kt + 1) & 1][ib] = halves_at(qt + 16 * ib * QTile::stride, 32 * (kt + 1), typed);
+            for (int ib = 0; ib < CT; ++ib) qf[(x + 1) & 1][ib] = operand(qt, q_at, 16 * ib, x + 1);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          if (!HELD) {
+            const Split<T, 2> s0(s[x][0]), s1(s[x][1]);
+#pragma unroll
+            for (int z = 0; z < PARTS; ++z) sp[0][z] = join(s0.part[z], s1.part[z]);
+          }
+#pragma unroll
+          for (int z = 0; z < PARTS; ++z)
+#pragma unroll
+            for (int ib = 0; ib < CT; ++ib) mma(o[ib], sp[HELD ? x : 0][z], qf[x & 1][ib]);
         }
-        __builtin_amdgcn_sched_barrier(0);
-        if (!HELD) {
-          const Split<T, 2> s0(s[2 * kt]), s1(s[2 * kt + 1]);
 #pragma unroll
-          for (int z = 0; z < PARTS; ++z) sp[0][z] = join(s0.part[z], s1.part[z]);
-        }
-#pragma unroll
-        for (int z = 0; z < PARTS; ++z)
-#pragma unroll
-          for (int ib = 0; ib < CT; ++ib) mma(o[ib], sp[HELD ? kt : 0][z], qf[kt & 1][ib]);
+        for (int ib = 0; ib < CT; ++ib) o[ib] *= reached[ib];
+        if (last) update(kv, n);
       }
-#pragma unroll
-      for (int ib = 0; ib < CT; ++ib) o[ib] *= reached[ib];
-      const bool last = g + 1 == a.rep, more = t + n < hi;
-      if (last) update(kv, n);
-      if (!last || more) qr.store(q_lds + (qb ^ 1) * Shape::q_bytes);
-      if (last && more) {
-        if (store_k(kv ^ 1)) not_finite[kv ^ 1] = 1;
-        const int after = t + n + tokens_at(t + n);
-        if (after < hi) load_k(after, tokens_at(after));
+      // P is whole; the next head's Q and, after the last head, the next chunk's K and V are here.  This head's Q and,
+      // after the last head, the chunk's K and V are read for the last time.
+      // What may still be on its way is what was asked for after that: the last head's rows of out, if they are known to
+      // be all, the Q for QBUF - 1 heads on, and K and V if they came before that.
+      constexpr int Q_LEFT = (QBUF - 2) * QN;
+      if (!q_new) {
+        arrive<0>();
+      } else if (QBUF > 2 && kv_new && !last) {
+        if (stored) arrive<KVN + Q_LEFT + CT>();
+        else arrive<KVN + Q_LEFT>();
+      } else {
+        if (stored) arrive<Q_LEFT + CT>();
+        else arrive<Q_LEFT>();
       }
-      fetch_next_q();
-      __syncthreads();
+      kv_new = last && fetch_kv(t + n + C, kv);
+      q_new = fetch_q();
       // ---- what the chunk's own tokens give
-      pair pf[CT][(CT + 1) / 2][PARTS];
+      if (!columns) {
+      } else if (!odd) {
+        pair pf[CT][CX][PARTS];
 #pragma unroll
-      for (int ib = 0; ib < CT; ++ib)
+        for (int ib = 0; ib < CT; ++ib)
 #pragma unroll
-        for (int jt = 0; jt <= ib; jt += 2)
+          for (int jx = 0; 2 * jx <= ib; ++jx)
 #pragma unroll
-          for (int z = 0; z < PARTS; ++z) pf[ib][jt / 2][z] = halves_at(pt + z * Shape::part_bytes + 16 * ib * PTile::stride, 16 * jt, typed);
-      __builtin_amdgcn_sched_barrier(0);
+            for (int z = 0; z < PARTS; ++z) pf[ib][jx][z] = operand(pt + z * Shape::part_bytes, p_at, 16 * ib, jx);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int jt = 0; jt < CT; jt += 2)
+        for (int jx = 0; jx < CX; ++jx)
 #pragma unroll
-        for (int z = 0; z < PARTS; ++z)
+          for (int z = 0; z < PARTS; ++z)
 #pragma unroll
-          for (int ib = jt; ib < CT; ++ib) mma(o[ib], join(vt[jt], vt[jt + 1]), pf[ib][jt / 2][z]);
+            for (int ib = 2 * jx; ib < CT; ++ib) mma(o[ib], vt[jx], pf[ib][jx][z]);
+      } else {
+        // a masked weight of zero times a value that is not finite would reach the tokens before it: only what a token
+        // sees is added, one by one
+#pragma unroll 1
+        for (int at = 0; at < C; ++at) {
+          const int j = summed<T>(at / 32, at / 16 % 2, at % 4, at / 4 % 4);
+          float mine = 0.f;
+#pragma unroll
+          for (int x = 0; x < 8 * CX; ++x) mine = x == at / 4 ? half_of(vt[x / 8], x / 4 % 2)[x % 4] : mine;
+          f32x4 v;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = __shfl(mine, 16 * (at % 4) + g4 + i);
+#pragma unroll
+          for (int ib = 0; ib < CT; ++ib) {
+            const int i = 16 * ib + l16;
+            float p = 0.f;
+#pragma unroll
+            for (int z = 0; z < PARTS; ++z) p += to_float(*reinterpret_cast<const T*>(pt + z * Shape::part_bytes + Tile<T, C>::at(i, j)));
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[ib][x] = j <= i ? fmaf(p, v[x], o[ib][x]) : o[ib][x];
+          }
+        }
+      }
       const int c = n0 + g4;
-      T* const o_at = out + t * a.out_stride + (int64_t)(h * a.rep + g) * d;
+      T* const o_at = out + t * a.out_stride + (int64_t)(h * a.rep + head) * d;
 #pragma unroll
       for (int ib = 0; ib < CT; ++ib) {
         const int i = 16 * ib + l16;
@@ -726,17 +888,18 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
           }
         }
       }
-      if (PBUF == 1) __syncthreads();              // P is free
+      stored = ALIGNED && n == C && columns;
+      if (PBUF == 1) arrive<63>();                 // P is free
       else pb ^= 1;
-      qb ^= 1;
+      qb = qb + 1 == QBUF ? 0 : qb + 1;
       if (last) {
         t += n;
         if (t >= hi) break;
-        n = tokens_at(t);
+        n = min(C, hi - t);
         kv ^= 1;
-        g = 0;
+        head = 0;
       } else {
-        ++g;
+        ++head;
       }
     }
   }
@@ -744,77 +907,90 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
   float* const s_to = STATES ? s_work : segment == segments - 1 && row != a.idle_row ? s_row : nullptr;
   if (s_to) {
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+    for (int x = 0; x < KX; ++x)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * kt + g4 + i, c = n0 + l16;
-        if (r < d && c < d) s_to[(int64_t)r * d + c] = s[kt][i];
-      }
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = dim_of<T>(x, y, g4 + i), c = n0 + l16;
+          if (r < d && c < d) s_to[(int64_t)r * d + c] = s[x][y][i];
+        }
   }
 }
 
+#define SCAN_AHEAD 16
+
 // What the segments add becomes the states at their starts, in place: one thread to 4 elements of a request's state.
-__global__ __launch_bounds__(256) void la_scan_kernel(LinearAttention a) {
+__global__ __launch_bounds__(64) void la_scan_kernel(LinearAttention a) {
   const int per_head = a.d * a.d / 4;
-  const int b = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
+  const int b = blockIdx.y, i = blockIdx.x * 64 + threadIdx.x;
   int lo, hi;
   bounds_of(a, b, lo, hi);
   const int segments = (hi - lo + a.segment - 1) / a.segment;
   const int row = a.rows[b];
   if (segments <= 1 || i >= a.nkv * per_head || row < 0 || row >= a.num_rows) return;
   const int h = i / per_head;
-  const float an = decay_power(a.log_decay[h], a.segment);
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  if (row != a.idle_row) s = *reinterpret_cast<const f32x4*>(a.state + (int64_t)row * a.state_stride + (int64_t)i * 4);
+  const float log_decay = a.log_decay[h];
+  f32x4 s = *reinterpret_cast<const f32x4*>(a.state + (int64_t)row * a.state_stride + (int64_t)i * 4);
   const int64_t unit = (int64_t)a.nkv * a.d * a.d;
   float* w = a.work + (int64_t)first_unit(a, b) * unit + (int64_t)i * 4;
-  for (int x = 0; x < segments; ++x, w += unit) {
-    f32x4 added = {0.f, 0.f, 0.f, 0.f};
-    if (x + 1 < segments) added = *reinterpret_cast<const f32x4*>(w);
-    *reinterpret_cast<f32x4*>(w) = s;
+  // SCAN_AHEAD at a time: their loads are on their way together (the last segment adds nothing that is needed)
+  float an = 0.f;
+  for (int x0 = 0; x0 < segments; x0 += SCAN_AHEAD) {
+    f32x4 added[SCAN_AHEAD];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) s[c] = fmaf(an, s[c], added[c]);
+    for (int x = 0; x < SCAN_AHEAD; ++x) added[x] = *reinterpret_cast<const f32x4*>(w + min(x0 + x, segments - 2) * unit);
+    if (x0 == 0) {
+      an = decay_power(log_decay, a.segment);
+      if (row == a.idle_row) s = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int x = 0; x < SCAN_AHEAD; ++x) {
+      if (x0 + x < segments) *reinterpret_cast<f32x4*>(w + (x0 + x) * unit) = s;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[c] = fmaf(an, s[c], added[x][c]);
+    }
   }
 }
 
-template <typename T, int DP, int WAVES, int C, int PBUF, bool STATES, bool ALIGNED, int PER_SIMD>
+template <typename T, int DP, int WAVES, int C, int QBUF, int PBUF, int KBUF, bool STATES, bool ALIGNED, int PER_SIMD>
 static int launch_chunks(const LinearAttention& a, int64_t units, hipStream_t stream) {
-  typedef ChunkShape<T, DP, WAVES, C, PBUF> Shape;
+  typedef ChunkShape<T, DP, WAVES, C, QBUF, PBUF, KBUF> Shape;
   static std::atomic<uint64_t> ready{0};           // devices on which the kernel may use this much LDS
   constexpr int bytes = Shape::lds(STATES);
   int device = 0;
   (void)hipGetDevice(&device);
   if (!((ready.load(std::memory_order_relaxed) >> (device & 63)) & 1)) {
-    hipError_t e = hipFuncSetAttribute((const void*)la_chunk_kernel<T, DP, WAVES, C, PBUF, STATES, ALIGNED, PER_SIMD>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    hipError_t e = hipFuncSetAttribute((const void*)la_chunk_kernel<T, DP, WAVES, C, QBUF, PBUF, KBUF, STATES, ALIGNED, PER_SIMD>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     MI_REQUIRE(e == hipSuccess, "linear attention: %d bytes of LDS: %s", bytes, hipGetErrorString(e));
     ready.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
   }
   const int64_t blocks = units * a.nkv * ((a.d + Shape::VS - 1) / Shape::VS);
   MI_REQUIRE(blocks <= 0x7fffffff, "linear attention: %lld workgroups are too many for one launch", (long long)blocks);
-  la_chunk_kernel<T, DP, WAVES, C, PBUF, STATES, ALIGNED, PER_SIMD><<<(uint32_t)blocks, Shape::threads, bytes, stream>>>(a);
+  la_chunk_kernel<T, DP, WAVES, C, QBUF, PBUF, KBUF, STATES, ALIGNED, PER_SIMD><<<(uint32_t)blocks, Shape::threads, bytes, stream>>>(a);
   MI_CHECK_LAUNCH("linear attention, chunks");
   return 0;
 }
 
-template <typename T, int DP, int WAVES, int C, int PBUF, bool ALIGNED, int PER_SIMD>
+template <typename T, int DP, int WAVES, int C, int QBUF, int PBUF, int KBUF, bool ALIGNED, int PER_SIMD>
 static int launch_aligned(const LinearAttention& a, hipStream_t stream) {
-  if (!a.segment) return launch_chunks<T, DP, WAVES, C, PBUF, false, ALIGNED, PER_SIMD>(a, a.num_requests, stream);
+  if (!a.segment) return launch_chunks<T, DP, WAVES, C, QBUF, PBUF, KBUF, false, ALIGNED, PER_SIMD>(a, a.num_requests, stream);
   const int64_t units = a.num_tokens / a.segment + a.num_requests;
-  if (launch_chunks<T, DP, WAVES, C, PBUF, true, ALIGNED, PER_SIMD>(a, units, stream)) return 1;
-  la_scan_kernel<<<dim3((a.nkv * a.d * a.d / 4 + 255) / 256, a.num_requests), 256, 0, stream>>>(a);
+  if (launch_chunks<T, DP, WAVES, C, QBUF, PBUF, KBUF, true, ALIGNED, PER_SIMD>(a, units, stream)) return 1;
+  la_scan_kernel<<<dim3((a.nkv * a.d * a.d / 4 + 63) / 64, a.num_requests), 64, 0, stream>>>(a);
   MI_CHECK_LAUNCH("linear attention, scan");
-  return launch_chunks<T, DP, WAVES, C, PBUF, false, ALIGNED, PER_SIMD>(a, units, stream);
+  return launch_chunks<T, DP, WAVES, C, QBUF, PBUF, KBUF, false, ALIGNED, PER_SIMD>(a, units, stream);
 }
 
-template <typename T, int DP, int WAVES, int C, int PBUF, int PER_SIMD>
+template <typename T, int DP, int WAVES, int C, int QBUF, int PBUF, int KBUF, int PER_SIMD>
 static int launch_prompt(const LinearAttention& a, hipStream_t stream) {
   auto fits = [](const void* p, int64_t stride, int bytes) {
     return ((uint64_t)p | (uint64_t)(stride * (int64_t)sizeof(T))) % bytes == 0 && stride * C * (int64_t)sizeof(T) < (1ll << 31);
   };
   const bool aligned = fits(a.q, a.q_stride, 16) && fits(a.k, a.k_stride, 16) && fits(a.v, a.v_stride, 16) &&
                        fits(a.out, a.out_stride, 4 * sizeof(T));
-  return aligned ? launch_aligned<T, DP, WAVES, C, PBUF, true, PER_SIMD>(a, stream)
-                 : launch_aligned<T, DP, WAVES, C, PBUF, false, 1>(a, stream);
+  return aligned ? launch_aligned<T, DP, WAVES, C, QBUF, PBUF, KBUF, true, PER_SIMD>(a, stream)
+                 : launch_aligned<T, DP, WAVES, C, QBUF, PBUF, KBUF, false, 1>(a, stream);
 }
 
 // segment: tokens of a segment (a multiple of 64), or 0 for one workgroup's walk over each whole request; work: then
@@ -826,14 +1002,14 @@ MI_EXPORT int mi_linear_attention(LA_ARGS, int segment, float* work, hipStream_t
   LinearAttention a = {q, k, v, out, state, rows, cu, log_decay, work, q_stride, k_stride, v_stride, out_stride, state_stride,
                        num_rows, idle_row, num_tokens, num_requests, nkv, nq / nkv, d, segment, scale};
   if (dtype == MI_DTYPE_BF16) {
-    if (d <= 64) return launch_prompt<bf16, 64, 4, LA_C64, LA_PBUF64, 2>(a, stream);
-    if (d <= 128) return launch_prompt<bf16, 128, 8, 64, 2, 2>(a, stream);
-    return launch_prompt<bf16, 256, 8, 32, 2, 2>(a, stream);
+    if (d <= 64) return launch_prompt<bf16, 64, 4, 32, 3, 2, 3, 2>(a, stream);
+    if (d <= 128) return launch_prompt<bf16, 128, 8, 64, 3, 2, 3, 2>(a, stream);
+    return launch_prompt<bf16, 256, 8, 32, 3, 2, 3, 2>(a, stream);
   }
   if (dtype == MI_DTYPE_F32) {
-    if (d <= 64) return launch_prompt<float, 64, 4, 32, 2, 2>(a, stream);
-    if (d <= 128) return launch_prompt<float, 128, 8, 32, 2, 2>(a, stream);
-    return launch_prompt<float, 256, 4, 32, 1, 1>(a, stream);
+    if (d <= 64) return launch_prompt<float, 64, 4, 32, 3, 2, 3, 2>(a, stream);
+    if (d <= 128) return launch_prompt<float, 128, 8, 32, 3, 2, 3, 2>(a, stream);
+    return launch_prompt<float, 256, 4, 32, 2, 1, 2, 1>(a, stream);
   }
   MI_FAIL("linear attention: dtype %d", dtype);
 }

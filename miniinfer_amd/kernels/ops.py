@@ -1194,15 +1194,18 @@ def _linear_attention_call(what, q, k, v, nq, nkv, d, out, state, state_rows, cu
           nq, nkv, d, log_decay.data_ptr(), scale)
 
 
-def linear_attention_segment(num_tokens: int, max_len: int, nkv: int, d: int, units: int = 256) -> int:
+def linear_attention_segment(num_tokens: int, num_requests: int, max_len: int, nkv: int, d: int, itemsize: int = 2,
+                             units: int = 256) -> int:
   """Tokens of a segment into which requests are cut, 0 for none: as many (whole chunks of 64) as make one workgroup for
-  every compute unit over all tokens.  A cut costs a pass over the keys and values for the segments' states and a kernel
-  that adds them up, so a longest request of up to three segments is left whole (24 requests of up to 950 tokens, 12 heads
-  of 80: 91 us whole, 101 in segments of 448; 8 requests of 1,024 tokens, 8 heads of 128: 246 us whole, 94 in segments of
-  256)."""
-  slices = -(-d // 128)
-  tokens = max(64, -(-num_tokens * nkv * slices // (units * 64)) * 64)
-  return tokens if max_len > 3 * tokens else 0
+  every compute unit over all tokens, two of the small ones of head sizes up to 64.  Every request's last segment may be a
+  short one, and a workgroup too many is a second turn on its compute unit, so they are counted, up to half of all (8
+  requests of 8,192 tokens together, 8 heads of 128: 67 us in segments of 384, 89 in segments of 256).  A cut costs a pass
+  over the keys and values for the segments' states and a kernel that adds them up, so a longest request of up to two
+  segments is left whole (24 requests of up to 950 tokens, 12 heads of 80: 74 us whole, 93 in segments of 384)."""
+  columns = 64 if d <= 64 or (itemsize == 4 and d > 128) else 128      # of a workgroup
+  workgroups = units * (2 if d <= 64 else 1) // (nkv * -(-d // columns))
+  tokens = max(64, -(-num_tokens // (64 * max(1, workgroups - num_requests + 1, workgroups // 2))) * 64)
+  return tokens if max_len > 2 * tokens else 0
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int, nkv: int, d: int, out: torch.Tensor,
@@ -1228,7 +1231,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int,
     raise KernelError(f"linear_attention: cu_q has {cu_q.numel()} entries for {state_rows.numel()} requests")
   with _on_device_of("linear_attention", q, k, v, out, state, state_rows, cu_q, log_decay) as stream:
     lib = _lib("linear_attention")
-    segment = linear_attention_segment(T, T if max_len is None else min(max_len, T), nkv, d, compute_units(q.get_device()))
+    segment = linear_attention_segment(T, state_rows.numel(), T if max_len is None else min(max_len, T), nkv, d,
+                                       q.element_size(), compute_units(q.get_device()))
     work = None
     if segment:
       work = torch.empty((T // segment + state_rows.numel()) * nkv * d * d, dtype=torch.float32, device=q.device)
