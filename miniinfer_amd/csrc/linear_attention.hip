@@ -561,20 +561,25 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
             out[(int64_t)t * a.out_stride + (int64_t)(h * a.rep + i / VS) * d + slice * VS + i % VS] = from_float<T>(NAN);
     return;
   }
-  if (tid <= C) {
-    const float p = decay_power(a.log_decay[h], tid);
-    power[tid] = p;
-    if (tid < C) left[C - 1 - tid] = p;
-  }
-  for (int i = C + tid; i < 2 * C; i += Shape::threads) left[i] = 0.f;
-  if (d < DP || d < (slice + 1) * VS)                    // columns past the end
+  if (d < DP || d < (slice + 1) * VS) {                  // columns past the end
     for (int i = tid; i < Shape::lds(STATES) / 16; i += Shape::threads) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
-  __syncthreads();
+    __syncthreads();
+  }
+  auto tables = [&]() {              // (after the first requests to memory: the exponentials take a while)
+    if (tid <= C) {
+      const float p = decay_power(a.log_decay[h], tid);
+      power[tid] = p;
+      if (tid < C) left[C - 1 - tid] = p;
+    }
+    for (int i = C + tid; i < 2 * C; i += Shape::threads) left[i] = 0.f;
+    __syncthreads();
+  };
 
   // the wave's columns of the state, accumulators (x, y): row dim_of(x, y, g4 + i), column n0 + l16
   f32x4 s[KX][2];
   float* const s_row = a.state + (int64_t)row * a.state_stride + (int64_t)h * d * d;
   float* const s_work = a.segment ? a.work + ((int64_t)unit * a.nkv + h) * d * d : nullptr;
+  float* const s_to = STATES ? s_work : segment == segments - 1 && row != a.idle_row ? s_row : nullptr;
   const float* const s_from = segments > 1 ? s_work : row == a.idle_row ? nullptr : s_row;
 
   const T* const kp = (const T*)a.k + (int64_t)h * d;
@@ -587,17 +592,28 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     k_way.template load<ALIGNED>(kp + t * a.k_stride, a.k_stride, n, k_lds + buf * Shape::q_bytes, wave, lane);
     v_way.template load<ALIGNED>(vp + t * a.v_stride, a.v_stride, n, v_lds + buf * Shape::v_bytes, wave, lane);
   };
+  // f(element of the wave's columns of the state, its place)
+  auto each_of_state = [&](auto f) {
+    auto walk = [&](int cols) {
+#pragma unroll
+      for (int x = 0; x < KX; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = dim_of<T>(x, y, i) + dim_of<T>(0, 0, g4);
+            if (r < cols) s[x][y][i] = f(s[x][y][i], (dim_of<T>(0, 0, g4) * cols + n0 + l16) + dim_of<T>(x, y, i) * cols);
+          }
+    };
+    if (d == DP) walk(DP);           // (the usual sizes: no checks, constant strides)
+    else if (n0 + l16 < d) walk(d);
+  };
   auto load_state = [&]() {
 #pragma unroll
     for (int x = 0; x < KX; ++x)
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = dim_of<T>(x, y, g4 + i), c = n0 + l16;
-          s[x][y][i] = 0.f;
-          if (!STATES && s_from && r < d && c < d) s[x][y][i] = s_from[(int64_t)r * d + c];
-        }
+      for (int y = 0; y < 2; ++y) s[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!STATES && s_from) each_of_state([&](float, int at) { return s_from[at]; });
   };
 
   const DownAt<T, DP> k_down(lane, 0);
@@ -658,6 +674,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     };
 #pragma unroll
     for (int i = 0; i + 1 < KBUF; ++i) fetch();
+    tables();
     if (next >= hi) arrive<0>();               // (at most KBUF - 1 chunks: all have to be here in the end)
     else arrive<(KBUF - 2) * KVN>();
     for (;;) {
@@ -704,6 +721,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     bool stored = false;                       // and whether CT stores to out came after it
 #pragma unroll
     for (int i = 1; i < QBUF; ++i) q_new = fetch_q();
+    tables();
     // the weights a^(i-j) of the P that the wave makes, and a^(i+1) of its tokens, both with the scale
     constexpr int PW = (CT * CX + WAVES - 1) / WAVES;
     int reach[PW];                   // i - j of a lane's first element: those of the next ones are less
@@ -815,7 +833,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
         }
 #pragma unroll
         for (int ib = 0; ib < CT; ++ib) o[ib] *= reached[ib];
-        if (last) update(kv, n);
+        if (last && (t + n < hi || s_to)) update(kv, n);
       }
       // P is whole; the next head's Q and, after the last head, the next chunk's K and V are here.  This head's Q and,
       // after the last head, the chunk's K and V are read for the last time.
@@ -904,18 +922,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     }
   }
 
-  float* const s_to = STATES ? s_work : segment == segments - 1 && row != a.idle_row ? s_row : nullptr;
-  if (s_to) {
-#pragma unroll
-    for (int x = 0; x < KX; ++x)
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = dim_of<T>(x, y, g4 + i), c = n0 + l16;
-          if (r < d && c < d) s_to[(int64_t)r * d + c] = s[x][y][i];
-        }
-  }
+  if (s_to) each_of_state([&](float e, int at) { return s_to[at] = e; });
 }
 
 #define SCAN_AHEAD 16
