@@ -435,6 +435,18 @@ struct Loader {
   }
 };
 
+// 16 bytes of a row from the accumulators of O^T.  In bfloat16 the lanes of two neighbouring groups of 16 change halves
+// between two accumulators, 4 columns of 16 rows each: one has then 8 columns of a row of the first, the other of the second.
+template <int CT>
+__device__ __forceinline__ u32x4 rows_of_out(int x, const f32x4 (&o)[CT], float) { return __builtin_bit_cast(u32x4, o[x]); }
+template <int CT>
+__device__ __forceinline__ u32x4 rows_of_out(int x, const f32x4 (&o)[CT], bf16) {
+  const mi_u32x2 p = __builtin_bit_cast(mi_u32x2, to_half(o[2 * x])), q = __builtin_bit_cast(mi_u32x2, to_half(o[2 * x + 1]));
+  const auto lo = __builtin_amdgcn_permlane16_swap(p[0], q[0], false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(p[1], q[1], false, false);
+  return u32x4{(uint32_t)lo[0], (uint32_t)hi[0], (uint32_t)lo[1], (uint32_t)hi[1]};
+}
+
 // All but the last `N` requests to memory of the wave are done, and every wave's LDS accesses; the waves meet.
 template <int N>
 __device__ __forceinline__ void arrive() {
@@ -500,8 +512,7 @@ struct ChunkShape {
 // 76 us, 114).
 //
 // STATES: only what a segment adds to its request's state (from zero), left in `work`; the last segment's is not needed.
-// ALIGNED: rows of q, k and v start at multiples of 16 bytes, of out at multiples of 4 elements, and a chunk of a tensor
-// spans less than 2^31 bytes.
+// ALIGNED: rows of q, k, v and out start at multiples of 16 bytes, and a chunk of a tensor spans less than 2^31 bytes.
 template <typename T, int DP, int WAVES, int C, int QBUF, int PBUF, int KBUF, bool STATES, bool ALIGNED, int PER_SIMD>
 __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAttention a) {
   typedef ChunkShape<T, DP, WAVES, C, QBUF, PBUF, KBUF> Shape;
@@ -691,7 +702,10 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       else arrive<0>();
     }
   } else {
-    const uint32_t out_offset = (uint32_t)((l16 * a.out_stride + n0 + g4) * (int)sizeof(T));
+    // the 16 bytes of a row of out that a lane writes (see rows_of_out)
+    constexpr int OUT_STEP = 4 / (int)sizeof(T), STORES = CT / OUT_STEP;
+    const int out_row = sizeof(T) == 2 ? 16 * (g & 1) + l16 : l16, out_col = n0 + (sizeof(T) == 2 ? 8 * (g >> 1) : g4);
+    const uint32_t out_offset = (uint32_t)((out_row * a.out_stride + out_col) * (int)sizeof(T));
     const OperandAt<T, DP> q_at(lane);
     const OperandAt<T, C> p_at(lane);
     // the query head whose Q is fetched next: head fg of tokens ft .. ft + fn - 1; Q goes round QBUF buffers
@@ -718,7 +732,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     load_state();
     const bool next_kv = fetch_kv(t + C, 1);
     bool q_new = false, kv_new = false;        // whether what was asked for last holds a Q, and K and V;
-    bool stored = false;                       // and whether CT stores to out came after it
+    bool stored = false;                       // and whether STORES to out came after it
 #pragma unroll
     for (int i = 1; i < QBUF; ++i) q_new = fetch_q();
     tables();
@@ -843,10 +857,10 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       if (!q_new) {
         arrive<0>();
       } else if (QBUF > 2 && kv_new && !last) {
-        if (stored) arrive<KVN + Q_LEFT + CT>();
+        if (stored) arrive<KVN + Q_LEFT + STORES>();
         else arrive<KVN + Q_LEFT>();
       } else {
-        if (stored) arrive<Q_LEFT + CT>();
+        if (stored) arrive<Q_LEFT + STORES>();
         else arrive<Q_LEFT>();
       }
       kv_new = last && fetch_kv(t + n + C, kv);
@@ -891,19 +905,21 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
           }
         }
       }
-      const int c = n0 + g4;
       T* const o_at = out + t * a.out_stride + (int64_t)(h * a.rep + head) * d;
+      if (ALIGNED) {
 #pragma unroll
-      for (int ib = 0; ib < CT; ++ib) {
-        const int i = 16 * ib + l16;
-        if (i < n && c < d) {
-          const float r[4] = {o[ib][0], o[ib][1], o[ib][2], o[ib][3]};
-          if (ALIGNED) {
-            store4((T*)((char*)(o_at + 16 * ib * a.out_stride) + out_offset), r);
-          } else {
+        for (int x = 0; x < STORES; ++x) {
+          const u32x4 r = rows_of_out(x, o, T{});
+          const int i = out_row + 16 * OUT_STEP * x;
+          if (i < n && out_col < d) *reinterpret_cast<u32x4*>((char*)(o_at + 16 * OUT_STEP * x * a.out_stride) + out_offset) = r;
+        }
+      } else {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) o_at[i * a.out_stride + c + x] = from_float<T>(r[x]);
-          }
+        for (int ib = 0; ib < CT; ++ib) {
+          const int i = 16 * ib + l16;
+          if (i < n && n0 + g4 < d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o_at[i * a.out_stride + n0 + g4 + x] = from_float<T>(o[ib][x]);
         }
       }
       stored = ALIGNED && n == C && columns;
@@ -995,7 +1011,7 @@ static int launch_prompt(const LinearAttention& a, hipStream_t stream) {
     return ((uint64_t)p | (uint64_t)(stride * (int64_t)sizeof(T))) % bytes == 0 && stride * C * (int64_t)sizeof(T) < (1ll << 31);
   };
   const bool aligned = fits(a.q, a.q_stride, 16) && fits(a.k, a.k_stride, 16) && fits(a.v, a.v_stride, 16) &&
-                       fits(a.out, a.out_stride, 4 * sizeof(T));
+                       fits(a.out, a.out_stride, 16);
   return aligned ? launch_aligned<T, DP, WAVES, C, QBUF, PBUF, KBUF, true, PER_SIMD>(a, stream)
                  : launch_aligned<T, DP, WAVES, C, QBUF, PBUF, KBUF, false, 1>(a, stream);
 }
