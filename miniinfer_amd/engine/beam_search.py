@@ -89,7 +89,8 @@ class BeamSearcher:
     return out
 
   def _fits(self, searches: Sequence[Search]) -> bool:
-    if len(searches) * self.params.num_beams > self.cache.num_free_slots():
+    beams = len(searches) * self.params.num_beams          # the tokens of a step
+    if beams > self.cache.num_free_slots() or beams > self.engine.config.max_num_batched_tokens:
       return False
     needs = [self._pages(s) for s in searches]
     return all(sum(n[gi] for n in needs) <= room for gi, room in enumerate(self.cache.room()))
@@ -174,7 +175,8 @@ class BeamSearcher:
       if not self._fits([s]):
         raise ValueError(f"a beam search of {self.params.num_beams} beams over a prompt of {len(s.prompt)} tokens plus "
                          f"max_tokens={s.max_tokens} does not fit the cache ({self._pages(s)} pages per group, "
-                         f"{self.cache.room()} free; {self.cache.num_free_slots()} request slots)")
+                         f"{self.cache.room()} free; {self.cache.num_free_slots()} request slots; steps of "
+                         f"{self.engine.config.max_num_batched_tokens} tokens)")
     try:
       while waiting:
         live = [waiting.pop(0)]

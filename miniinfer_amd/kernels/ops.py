@@ -1175,6 +1175,8 @@ def _linear_attention_call(what, q, k, v, nq, nkv, d, out, state, state_rows, cu
   op, os = _linear_attention_rows(what, "out", out, T, nqd, dtype)
   if out.shape[1] != nqd:
     raise KernelError(f"{what}: out {tuple(out.shape)} is not [{T}, {nqd}]")
+  if T and op in (qp, kp, vp):
+    raise KernelError(f"{what}: out shares memory with an input")
   shape, stride, sp = state.shape, state.stride(), state.data_ptr()
   if state.dtype is not torch.float32 or len(shape) != 4 or shape[1:] != (nkv, d, d) or stride[2:] != (d, 1) \
       or (nkv > 1 and stride[1] != d * d):
@@ -1215,14 +1217,15 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int,
 
       S_t = a S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t,   a = exp(log_decay[kv head])
 
-  q [T, >= nq*d], k, v [T, >= nkv*d] rows (the parts of a fused q|k|v buffer are fine), out [T, nq*d]; nq / nkv query
-  heads share a kv head's state.  state float32 [rows, nkv, d, d] (key dim, value dim) is read at state_rows[b] and left
-  there as it is after request b's last token; requests of one call have rows of their own.  idle_row: a row that stands
-  for none; requests on it, any number, start from zeros and leave nothing (the padding entries of captured steps).  cu_q int32 [B + 1] = first
-  token of each request: a request without tokens leaves its state as it is, rows of `out` that belong to no request are
-  left as they are, and a state row outside the buffer gives rows of NaN.  log_decay float32 [nkv], <= 0 (-inf: a = 0)
-  or positive for a growing state.  max_len: the most tokens of one request if the host knows it (default: T); it only
-  chooses how the work is cut.  float32 and bfloat16; states and sums are 32-bit."""
+  q [T, >= nq*d], k, v [T, >= nkv*d] rows (the parts of a fused q|k|v buffer are fine), out [T, nq*d] in memory of its
+  own; nq / nkv query heads share a kv head's state.  state float32 [rows, nkv, d, d] (key dim, value dim) is read at
+  state_rows[b] and left there as it is after request b's last token; requests of one call have rows of their own.
+  idle_row: a row that stands for none; requests on it, any number, start from zeros and leave nothing (the padding
+  entries of captured steps).  cu_q int32 [B + 1] = first token of each request: a request without tokens leaves its
+  state as it is, rows of `out` that belong to no request are left as they are, and a state row outside the buffer gives
+  rows of NaN.  log_decay float32 [nkv], <= 0 (-inf: a = 0) or positive for a growing state.  max_len: the most tokens of
+  one request if the host knows it (default: T); it only chooses how the work is cut.  float32 and bfloat16; states and
+  sums are 32-bit."""
   args = _linear_attention_call("linear_attention", q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay, scale,
                                 idle_row)
   _i32("cu_q", cu_q)
@@ -1267,8 +1270,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_beams: int,
       scores[b] + logits[b, v] - log sum_u exp(logits[b, u])      b over the group's beams, v over the vocabulary
 
   the largest, largest first, equal ones by (beam, token).  logits float32 [G * num_beams, V] with dense rows, scores
-  float32 [G * num_beams] (-inf, or anything else that is not finite: a beam that does not take part).  Returns (scores float32, beams int32 in
-  0 .. num_beams - 1, tokens int32), each [G, count].  A logit that is NaN counts as -inf; where a row holds +inf, those
+  float32 [G * num_beams] (-inf, or anything else that is not finite: a beam that does not take part).  Returns (scores
+  float32, beams int32 in 0 .. num_beams - 1, tokens int32), each [G, count].  A logit that is NaN counts as -inf; where a row holds +inf, those
   tokens share its mass; a row of -inf only has no candidate above -inf.  If fewer than `count` candidates are above -inf
   the rest of the list has score -inf.  Sums of exponentials and the scores that are compared are 64-bit."""
   if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
@@ -1305,8 +1308,8 @@ MOVE_ROWS_MAX = 16384        # moves of a call: one workgroup holds a piece of e
 def move_rows(buffers, src: torch.Tensor, dst: torch.Tensor) -> None:
   """In place, in every layer of every buffer: row dst[i] becomes what row src[i] was before the call, for all i as if
   at once (permutations and cycles are fine; a row may be a source more than once, a destination only once).  buffers: a
-  tensor or up to 8 of them, [layers, rows, ...] with dense rows, of any dtype: a cache group's key and value pages, a
-  group's states.  src, dst: int32 [n] on the device, n up to 16,384; entries outside a buffer's rows move nothing there
+  tensor or up to 8 of them that share no memory, [layers, rows, ...] with dense rows, of any dtype: a cache group's key
+  and value pages, a group's states.  src, dst: int32 [n] on the device, n up to 16,384; entries outside a buffer's rows move nothing there
   (pad with -1)."""
   buffers = [buffers] if isinstance(buffers, torch.Tensor) else list(buffers)
   if not 1 <= len(buffers) <= MOVE_ROWS_MAX_BUFFERS:
@@ -1333,6 +1336,8 @@ def move_rows(buffers, src: torch.Tensor, dst: torch.Tensor) -> None:
       per_layer = t.stride(0) if layers > 1 else row
       per_row = t.stride(1) if rows > 1 else row
     spec += (t.data_ptr(), per_layer * size, per_row * size, row * size, layers, rows)
+  if len(set(spec[::6])) != len(spec) // 6:
+    raise KernelError("move_rows: a buffer is given twice")
   n = src.numel()
   if src.dtype is not torch.int32 or dst.dtype is not torch.int32 or not src.is_contiguous() or not dst.is_contiguous():
     _i32("src", src)
