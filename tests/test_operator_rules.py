@@ -63,7 +63,8 @@ def test_move_rows_refuses_a_buffer_twice():
 @pytest.mark.parametrize("tokens,slots,fits", [(64, 8, True), (4, 8, True), (3, 8, False), (64, 3, False)])
 def test_a_search_needs_a_slot_and_a_token_of_a_step_for_each_beam(tokens, slots, fits):
   need = FixedState(shape=(1, 2, 2), dtype=torch.float32)
-  cache = CacheManager([need], page_size=4, num_pages=8, max_requests=slots, dtype=torch.float32, device="cpu")
+  cache = CacheManager([need], page_size=4, num_pages=8, max_requests=slots, max_model_len=16,
+                       dtype=torch.float32, device="cpu")
   engine = SimpleNamespace(cache=cache, runner=None, scheduler=SimpleNamespace(eos_token_ids=[]),
                            config=SimpleNamespace(max_num_batched_tokens=tokens))
   searcher = BeamSearcher(engine, BeamSearchParams(num_beams=4, max_tokens=2))
