@@ -194,12 +194,12 @@ MI_EXPORT int mi_linear_attention_step(LA_ARGS, hipStream_t stream) {
 // first and last 4 are a "half".  An accumulator's lane has column l % 16 and rows 4 g .. 4 g + 3, so that two
 // accumulators are the two halves of an operand: for S, whose rows are given out accordingly (`dim_of`).
 //
-// Q, K and V go straight from memory to LDS (lane i's 16 bytes land at base + 16 i), in tiles of whole rows, two chunks of
-// K and V and the Q of three query heads at a time, with the waits written out by count.  The piece of 16 bytes that a
-// lane asks for is chosen such that piece p of row r lies at place p ^ swap(r): then the operands' reads, 16 pieces at a
-// time (lanes 0-3, 12-15 and 20-27, ...), and the transposing reads, 16 times 8 bytes of 4 rows, meet no bank twice
-// (with p ^ 2 (r mod 4), as good for the former alone, the LDS was busy twice as long, and 32,768 tokens of 32 heads on
-// 8 of 128 took 209 us instead of 198, without the kernels for segments).
+// Q, K and V go straight from memory to LDS (lane i's 16 bytes land at base + 16 i), in tiles of whole rows, two of each:
+// one is worked on while the other one is filled (three made no difference); the waits are written out by count.  The
+// piece of 16 bytes that a lane asks for is chosen such that piece p of row r lies at place p ^ swap(r): then the
+// operands' reads, 16 pieces at a time (lanes 0-3, 12-15 and 20-27, ...), and the transposing reads, 16 times 8 bytes of
+// 4 rows, meet no bank twice (with p ^ 2 (r mod 4), as good for the former alone, the LDS was busy twice as long, and
+// 32,768 tokens of 32 heads on 8 of 128 took 209 us instead of 198, without the kernels for segments).
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -491,8 +491,8 @@ __device__ __forceinline__ int first_unit(const LinearAttention& a, int b) {
   return min(max(a.cu[b], 0), a.num_tokens) / a.segment + b;
 }
 
-// QBUF, PBUF, KBUF: buffers of Q, of P and, for the segments' states, of K and V (2 otherwise).
-template <typename T, int DP, int WAVES, int C, int QBUF, int PBUF, int KBUF>
+// PBUF: buffers of P.
+template <typename T, int DP, int WAVES, int C, int PBUF>
 struct ChunkShape {
   static constexpr int waves = WAVES, threads = 64 * WAVES;
   static constexpr int VS = 16 * waves;
@@ -500,22 +500,22 @@ struct ChunkShape {
   static constexpr int q_bytes = C * Tile<T, DP>::stride, v_bytes = C * Tile<T, VS>::stride;
   static constexpr int part_bytes = C * Tile<T, C>::stride, p_bytes = parts * part_bytes;
   static constexpr int lds(bool states) {
-    return states ? KBUF * (q_bytes + v_bytes) : 2 * (q_bytes + v_bytes) + QBUF * q_bytes + PBUF * p_bytes;
+    return 2 * (q_bytes + v_bytes) + (states ? 0 : 2 * q_bytes + PBUF * p_bytes);
   }
 };
 
-// What bounds it (that workload, 198 us at 3.4 TB/s): the matrix cores are busy for 30% of the time, the vector ALUs and the
-// LDS for about as long, memory for half of it.  With 8 waves on a compute unit, all that the registers (256) and the LDS
-// (144 KB) allow, the waits between a head's products are not covered: without loads and stores it takes 142 us, without
-// stores 25 less, without any one of the products 0 to 17 less.  Smaller chunks (32 tokens) with twice the workgroups are
-// slower with heads of 128 (256 us for the whole call, 234) and faster with heads up to 64 (8,192 tokens, 32 heads:
-// 76 us, 114).
+// What bounds it (that workload, 192 us at 3.5 TB/s): the matrix cores are busy for 30% of the time, the vector ALUs and
+// the LDS for about as long, memory for half of it.  With 8 waves on a compute unit, all that the registers (256) and the
+// LDS (128 KB) allow, the waits between a head's products are not covered: without loads and stores it takes 142 us,
+// without stores 25 less, without any one of the products 0 to 17 less.  Chunks of 32 tokens are slower with heads of 128
+// (258 us for the whole call, 234 with 64) and quicker with heads up to 64, where several workgroups share a compute unit
+// (8,192 tokens, 32 heads: 76 us, 114 with 64).
 //
 // STATES: only what a segment adds to its request's state (from zero), left in `work`; the last segment's is not needed.
 // ALIGNED: rows of q, k, v and out start at multiples of 16 bytes, and a chunk of a tensor spans less than 2^31 bytes.
-template <typename T, int DP, int WAVES, int C, int QBUF, int PBUF, int KBUF, bool STATES, bool ALIGNED, int PER_SIMD>
+template <typename T, int DP, int WAVES, int C, int PBUF, bool STATES, bool ALIGNED, int PER_SIMD>
 __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAttention a) {
-  typedef ChunkShape<T, DP, WAVES, C, QBUF, PBUF, KBUF> Shape;
+  typedef ChunkShape<T, DP, WAVES, C, PBUF> Shape;
   typedef typename Half<T>::type half;
   typedef typename Half<T>::pair pair;
   constexpr int PARTS = Shape::parts, KX = DP / 32, KB = KX < 4 ? KX : 4, CX = C / 32, CT = C / 16, VS = Shape::VS;
@@ -524,9 +524,9 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
   __shared__ float left[2 * C];      // a^(C-1-i), zeros from C on
   __shared__ int found;
   char* const k_lds = lds;
-  char* const v_lds = k_lds + (STATES ? KBUF : 2) * Shape::q_bytes;
-  char* const q_lds = v_lds + (STATES ? KBUF : 2) * Shape::v_bytes;
-  char* const p_lds = q_lds + QBUF * Shape::q_bytes;
+  char* const v_lds = k_lds + 2 * Shape::q_bytes;
+  char* const q_lds = v_lds + 2 * Shape::v_bytes;
+  char* const p_lds = q_lds + 2 * Shape::q_bytes;
 
   const int tid = threadIdx.x, lane = tid & (MI_WAVE - 1), l16 = lane & 15, g = lane / 16, g4 = 4 * g;
   const int wave = __builtin_amdgcn_readfirstlane(tid / MI_WAVE);
@@ -598,7 +598,6 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
   const T* const qp = (const T*)a.q + (int64_t)h * a.rep * d;
   const Loader<T, DP, C, WAVES> k_way(wave, lane, a.k_stride, d), q_way(wave, lane, a.q_stride, d);
   const Loader<T, VS, C, WAVES> v_way(wave, lane, a.v_stride, d - slice * VS);
-  constexpr int QN = ALIGNED ? q_way.count : 0, KVN = ALIGNED ? k_way.count + v_way.count : 0;     // requests of a wave
   auto load_kv = [&](int t, int n, int buf) {
     k_way.template load<ALIGNED>(kp + t * a.k_stride, a.k_stride, n, k_lds + buf * Shape::q_bytes, wave, lane);
     v_way.template load<ALIGNED>(vp + t * a.v_stride, a.v_stride, n, v_lds + buf * Shape::v_bytes, wave, lane);
@@ -673,33 +672,22 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
   // The chunk at hand has the n tokens from t on.
   int t = lo, n = min(C, hi - lo), kv = 0;
   if constexpr (STATES) {
-    // chunks go round KBUF buffers: KBUF - 1 are on their way while one is worked on
-    load_state();
-    int next = lo, slot = 0;
-    auto fetch = [&]() {
-      if (next >= hi) return false;
-      load_kv(next, min(C, hi - next), slot);
-      next += C;
-      slot = slot + 1 == KBUF ? 0 : slot + 1;
-      return true;
-    };
-#pragma unroll
-    for (int i = 0; i + 1 < KBUF; ++i) fetch();
+    load_state();                    // (zeros)
+    load_kv(t, n, 0);
     tables();
-    if (next >= hi) arrive<0>();               // (at most KBUF - 1 chunks: all have to be here in the end)
-    else arrive<(KBUF - 2) * KVN>();
+    arrive<0>();
     for (;;) {
-      const bool more = fetch();
+      const bool more = t + n < hi;
+      if (more) load_kv(t + n, min(C, hi - t - n), kv ^ 1);
       if (columns) {
         read_v(kv, n);
         update(kv, n);
       }
+      if (!more) break;
+      arrive<0>();
       t += n;
-      if (t >= hi) break;
       n = min(C, hi - t);
-      kv = kv + 1 == KBUF ? 0 : kv + 1;
-      if (more) arrive<(KBUF - 2) * KVN>();
-      else arrive<0>();
+      kv ^= 1;
     }
   } else {
     // the 16 bytes of a row of out that a lane writes (see rows_of_out)
@@ -708,33 +696,26 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     const uint32_t out_offset = (uint32_t)((out_row * a.out_stride + out_col) * (int)sizeof(T));
     const OperandAt<T, DP> q_at(lane);
     const OperandAt<T, C> p_at(lane);
-    // the query head whose Q is fetched next: head fg of tokens ft .. ft + fn - 1; Q goes round QBUF buffers
+    // the query head whose Q is fetched next: head fg of tokens ft .. ft + fn - 1
     int ft = t, fn = n, fg = 0, slot = 0;
     auto fetch_q = [&]() {
-      if (ft >= hi) return false;
+      if (ft >= hi) return;
       q_way.template load<ALIGNED>(qp + ft * a.q_stride + fg * d, a.q_stride, fn, q_lds + slot * Shape::q_bytes, wave, lane);
-      slot = slot + 1 == QBUF ? 0 : slot + 1;
+      slot ^= 1;
       if (++fg == a.rep) {
         fg = 0;
         ft += fn;
         fn = min(C, hi - ft);
       }
-      return true;
     };
-    // K and V: the chunk after next is asked for at the end of a chunk
     auto fetch_kv = [&](int from, int buf) {
-      if (from >= hi) return false;
-      load_kv(from, min(C, hi - from), buf);
-      return true;
+      if (from < hi) load_kv(from, min(C, hi - from), buf);
     };
     load_kv(t, n, 0);
     fetch_q();
     load_state();
-    const bool next_kv = fetch_kv(t + C, 1);
-    bool q_new = false, kv_new = false;        // whether what was asked for last holds a Q, and K and V;
-    bool stored = false;                       // and whether STORES to out came after it
-#pragma unroll
-    for (int i = 1; i < QBUF; ++i) q_new = fetch_q();
+    fetch_kv(t + C, 1);
+    fetch_q();
     tables();
     // the weights a^(i-j) of the P that the wave makes, and a^(i+1) of its tokens, both with the scale
     constexpr int PW = (CT * CX + WAVES - 1) / WAVES;
@@ -757,8 +738,8 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     constexpr bool HELD = DP <= 128;
     pair sp[HELD ? KX : 1][PARTS];
     bool odd = false;                // whether one of the wave's values is not finite
-    if (next_kv && q_new) arrive<KVN + (QBUF - 1) * QN>();
-    else arrive<0>();
+    bool stored = false;             // whether the last head's rows of out are known to be STORES stores of the wave
+    arrive<0>();
     // (the state is here: else the compiler would wait for it, and for all that came after it, in every turn)
 #pragma unroll
     for (int x = 0; x < KX; ++x)
@@ -849,22 +830,13 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
         for (int ib = 0; ib < CT; ++ib) o[ib] *= reached[ib];
         if (last && (t + n < hi || s_to)) update(kv, n);
       }
-      // P is whole; the next head's Q and, after the last head, the next chunk's K and V are here.  This head's Q and,
-      // after the last head, the chunk's K and V are read for the last time.
-      // What may still be on its way is what was asked for after that: the last head's rows of out, if they are known to
-      // be all, the Q for QBUF - 1 heads on, and K and V if they came before that.
-      constexpr int Q_LEFT = (QBUF - 2) * QN;
-      if (!q_new) {
-        arrive<0>();
-      } else if (QBUF > 2 && kv_new && !last) {
-        if (stored) arrive<KVN + Q_LEFT + STORES>();
-        else arrive<KVN + Q_LEFT>();
-      } else {
-        if (stored) arrive<Q_LEFT + STORES>();
-        else arrive<Q_LEFT>();
-      }
-      kv_new = last && fetch_kv(t + n + C, kv);
-      q_new = fetch_q();
+      // P is whole; the next head's Q and, after the last head, the next chunk's K and V are here: all that was asked for
+      // but the last head's rows of out, which went off after it.  This head's Q and, after the last head, the chunk's K
+      // and V are read for the last time, so that their places take the Q of the head after next and the chunk after next.
+      if (stored) arrive<STORES>();
+      else arrive<0>();
+      if (last) fetch_kv(t + n + C, kv);
+      fetch_q();
       // ---- what the chunk's own tokens give
       if (!columns) {
       } else if (!odd) {
@@ -925,7 +897,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       stored = ALIGNED && n == C && columns;
       if (PBUF == 1) arrive<63>();                 // P is free
       else pb ^= 1;
-      qb = qb + 1 == QBUF ? 0 : qb + 1;
+      qb ^= 1;
       if (last) {
         t += n;
         if (t >= hi) break;
@@ -976,44 +948,44 @@ __global__ __launch_bounds__(64) void la_scan_kernel(LinearAttention a) {
   }
 }
 
-template <typename T, int DP, int WAVES, int C, int QBUF, int PBUF, int KBUF, bool STATES, bool ALIGNED, int PER_SIMD>
+template <typename T, int DP, int WAVES, int C, int PBUF, bool STATES, bool ALIGNED, int PER_SIMD>
 static int launch_chunks(const LinearAttention& a, int64_t units, hipStream_t stream) {
-  typedef ChunkShape<T, DP, WAVES, C, QBUF, PBUF, KBUF> Shape;
+  typedef ChunkShape<T, DP, WAVES, C, PBUF> Shape;
   static std::atomic<uint64_t> ready{0};           // devices on which the kernel may use this much LDS
   constexpr int bytes = Shape::lds(STATES);
   int device = 0;
   (void)hipGetDevice(&device);
   if (!((ready.load(std::memory_order_relaxed) >> (device & 63)) & 1)) {
-    hipError_t e = hipFuncSetAttribute((const void*)la_chunk_kernel<T, DP, WAVES, C, QBUF, PBUF, KBUF, STATES, ALIGNED, PER_SIMD>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    hipError_t e = hipFuncSetAttribute((const void*)la_chunk_kernel<T, DP, WAVES, C, PBUF, STATES, ALIGNED, PER_SIMD>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     MI_REQUIRE(e == hipSuccess, "linear attention: %d bytes of LDS: %s", bytes, hipGetErrorString(e));
     ready.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
   }
   const int64_t blocks = units * a.nkv * ((a.d + Shape::VS - 1) / Shape::VS);
   MI_REQUIRE(blocks <= 0x7fffffff, "linear attention: %lld workgroups are too many for one launch", (long long)blocks);
-  la_chunk_kernel<T, DP, WAVES, C, QBUF, PBUF, KBUF, STATES, ALIGNED, PER_SIMD><<<(uint32_t)blocks, Shape::threads, bytes, stream>>>(a);
+  la_chunk_kernel<T, DP, WAVES, C, PBUF, STATES, ALIGNED, PER_SIMD><<<(uint32_t)blocks, Shape::threads, bytes, stream>>>(a);
   MI_CHECK_LAUNCH("linear attention, chunks");
   return 0;
 }
 
-template <typename T, int DP, int WAVES, int C, int QBUF, int PBUF, int KBUF, bool ALIGNED, int PER_SIMD>
+template <typename T, int DP, int WAVES, int C, int PBUF, bool ALIGNED, int PER_SIMD>
 static int launch_aligned(const LinearAttention& a, hipStream_t stream) {
-  if (!a.segment) return launch_chunks<T, DP, WAVES, C, QBUF, PBUF, KBUF, false, ALIGNED, PER_SIMD>(a, a.num_requests, stream);
+  if (!a.segment) return launch_chunks<T, DP, WAVES, C, PBUF, false, ALIGNED, PER_SIMD>(a, a.num_requests, stream);
   const int64_t units = a.num_tokens / a.segment + a.num_requests;
-  if (launch_chunks<T, DP, WAVES, C, QBUF, PBUF, KBUF, true, ALIGNED, PER_SIMD>(a, units, stream)) return 1;
+  if (launch_chunks<T, DP, WAVES, C, PBUF, true, ALIGNED, PER_SIMD>(a, units, stream)) return 1;
   la_scan_kernel<<<dim3((a.nkv * a.d * a.d / 4 + 63) / 64, a.num_requests), 64, 0, stream>>>(a);
   MI_CHECK_LAUNCH("linear attention, scan");
-  return launch_chunks<T, DP, WAVES, C, QBUF, PBUF, KBUF, false, ALIGNED, PER_SIMD>(a, units, stream);
+  return launch_chunks<T, DP, WAVES, C, PBUF, false, ALIGNED, PER_SIMD>(a, units, stream);
 }
 
-template <typename T, int DP, int WAVES, int C, int QBUF, int PBUF, int KBUF, int PER_SIMD>
+template <typename T, int DP, int WAVES, int C, int PBUF, int PER_SIMD>
 static int launch_prompt(const LinearAttention& a, hipStream_t stream) {
   auto fits = [](const void* p, int64_t stride, int bytes) {
     return ((uint64_t)p | (uint64_t)(stride * (int64_t)sizeof(T))) % bytes == 0 && stride * C * (int64_t)sizeof(T) < (1ll << 31);
   };
   const bool aligned = fits(a.q, a.q_stride, 16) && fits(a.k, a.k_stride, 16) && fits(a.v, a.v_stride, 16) &&
                        fits(a.out, a.out_stride, 16);
-  return aligned ? launch_aligned<T, DP, WAVES, C, QBUF, PBUF, KBUF, true, PER_SIMD>(a, stream)
-                 : launch_aligned<T, DP, WAVES, C, QBUF, PBUF, KBUF, false, 1>(a, stream);
+  return aligned ? launch_aligned<T, DP, WAVES, C, PBUF, true, PER_SIMD>(a, stream)
+                 : launch_aligned<T, DP, WAVES, C, PBUF, false, 1>(a, stream);
 }
 
 // segment: tokens of a segment (a multiple of 64), or 0 for one workgroup's walk over each whole request; work: then
@@ -1025,14 +997,14 @@ MI_EXPORT int mi_linear_attention(LA_ARGS, int segment, float* work, hipStream_t
   LinearAttention a = {q, k, v, out, state, rows, cu, log_decay, work, q_stride, k_stride, v_stride, out_stride, state_stride,
                        num_rows, idle_row, num_tokens, num_requests, nkv, nq / nkv, d, segment, scale};
   if (dtype == MI_DTYPE_BF16) {
-    if (d <= 64) return launch_prompt<bf16, 64, 4, 32, 3, 2, 3, 2>(a, stream);
-    if (d <= 128) return launch_prompt<bf16, 128, 8, 64, 3, 2, 3, 2>(a, stream);
-    return launch_prompt<bf16, 256, 8, 32, 3, 2, 3, 2>(a, stream);
+    if (d <= 64) return launch_prompt<bf16, 64, 4, 32, 2, 2>(a, stream);
+    if (d <= 128) return launch_prompt<bf16, 128, 8, 64, 2, 2>(a, stream);
+    return launch_prompt<bf16, 256, 8, 32, 2, 2>(a, stream);
   }
   if (dtype == MI_DTYPE_F32) {
-    if (d <= 64) return launch_prompt<float, 64, 4, 32, 3, 2, 3, 2>(a, stream);
-    if (d <= 128) return launch_prompt<float, 128, 8, 32, 3, 2, 3, 2>(a, stream);
-    return launch_prompt<float, 256, 4, 32, 2, 1, 2, 1>(a, stream);
+    if (d <= 64) return launch_prompt<float, 64, 4, 32, 2, 2>(a, stream);
+    if (d <= 128) return launch_prompt<float, 128, 8, 32, 2, 2>(a, stream);
+    return launch_prompt<float, 256, 4, 32, 1, 1>(a, stream);
   }
   MI_FAIL("linear attention: dtype %d", dtype);
 }
