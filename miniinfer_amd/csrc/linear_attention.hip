@@ -766,7 +766,9 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       const char* const qt = q_lds + qb * Shape::q_bytes;
       const char* const kt = k_lds + kv * Shape::q_bytes;
       char* const pt = p_lds + pb * Shape::p_bytes;
-      // ---- P^T: to a wave 16 queries and 32 tokens, or that again for the next waves' worth of them
+      // ---- P^T: to a wave 16 queries and 32 tokens, or that again for the next waves' worth of them.  All waves wait for
+      // it, so it goes before the other wave's products (32,768 tokens 229 us, without that 233)
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int y = 0; y < PW; ++y) {
         const int x = wave + y * WAVES, ib = x % CT, jx = x / CT;
@@ -801,6 +803,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
           *reinterpret_cast<half*>(at + Tile<T, C>::at(16 * ib + l16, 32 * jx + 16 + g4)) = s1.part[z];
         }
       }
+      __builtin_amdgcn_s_setprio(0);
       // ---- what the state gives
       f32x4 o[CT];
 #pragma unroll
