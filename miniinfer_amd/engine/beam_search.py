@@ -72,7 +72,10 @@ class BeamSearcher:
       stop |= set(engine.scheduler.eos_token_ids)
     self.stop = stop
     # enough candidates that num_beams of them go on whatever the others end with
-    self.count = min(ops.BEAM_MAX_COUNT, (1 + max(1, len(stop))) * params.num_beams)
+    self.count = (1 + len(stop)) * params.num_beams
+    if self.count > ops.BEAM_MAX_COUNT:
+      raise ValueError(f"num_beams={params.num_beams} with {len(stop)} tokens that end a hypothesis: at most "
+                       f"{ops.BEAM_MAX_COUNT // (1 + len(stop))} are supported")
 
   # ------------------------------------------------------------------ requests
   def _new_request(self) -> Tuple:

@@ -73,3 +73,15 @@ def test_a_search_needs_a_slot_and_a_token_of_a_step_for_each_beam(tokens, slots
   if not fits:
     with pytest.raises(ValueError, match="does not fit"):
       searcher.run([[1, 2, 3]])
+
+
+@pytest.mark.parametrize("eos,stop,ignore,most", [([], [], False, 64), ([7], [], False, 32), ([7, 9], [], False, 21),
+                                                  ([7, 9], [9, 11, 12], False, 12), ([7, 9], [], True, 64)])
+def test_a_search_has_candidates_for_every_beam_whatever_ends(eos, stop, ignore, most):
+  """Of the candidates, every beam may bring every token that ends it; num_beams others have to be left."""
+  engine = SimpleNamespace(cache=None, runner=None, config=None, scheduler=SimpleNamespace(eos_token_ids=eos))
+  new = lambda n: BeamSearcher(engine, BeamSearchParams(num_beams=n, stop_token_ids=stop, ignore_eos=ignore))
+  assert new(most).count <= ops.BEAM_MAX_COUNT
+  assert new(most).count >= most * (1 + len(set(stop) | (set() if ignore else set(eos))))
+  with pytest.raises(ValueError, match="at most"):
+    new(most + 1)
