@@ -840,6 +840,25 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       else arrive<0>();
       if (last) fetch_kv(t + n + C, kv);
       fetch_q();
+      auto store = [&]() {
+        T* const o_at = out + t * a.out_stride + (int64_t)(h * a.rep + head) * d;
+        if (ALIGNED) {
+#pragma unroll
+          for (int x = 0; x < STORES; ++x) {
+            const u32x4 r = rows_of_out(x, o, T{});
+            const int i = out_row + 16 * OUT_STEP * x;
+            if (i < n && out_col < d) *reinterpret_cast<u32x4*>((char*)(o_at + 16 * OUT_STEP * x * a.out_stride) + out_offset) = r;
+          }
+        } else {
+#pragma unroll
+          for (int ib = 0; ib < CT; ++ib) {
+            const int i = 16 * ib + l16;
+            if (i < n && n0 + g4 < d)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o_at[i * a.out_stride + n0 + g4 + x] = from_float<T>(o[ib][x]);
+          }
+        }
+      };
       // ---- what the chunk's own tokens give
       if (!columns) {
       } else if (!odd) {
@@ -857,6 +876,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
           for (int z = 0; z < PARTS; ++z)
 #pragma unroll
             for (int ib = 2 * jx; ib < CT; ++ib) mma(o[ib], vt[jx], pf[ib][jx][z]);
+        store();
       } else {
         // a masked weight of zero times a value that is not finite would reach the tokens before it: only what a token
         // sees is added, one by one
@@ -879,23 +899,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
             for (int x = 0; x < 4; ++x) o[ib][x] = j <= i ? fmaf(p, v[x], o[ib][x]) : o[ib][x];
           }
         }
-      }
-      T* const o_at = out + t * a.out_stride + (int64_t)(h * a.rep + head) * d;
-      if (ALIGNED) {
-#pragma unroll
-        for (int x = 0; x < STORES; ++x) {
-          const u32x4 r = rows_of_out(x, o, T{});
-          const int i = out_row + 16 * OUT_STEP * x;
-          if (i < n && out_col < d) *reinterpret_cast<u32x4*>((char*)(o_at + 16 * OUT_STEP * x * a.out_stride) + out_offset) = r;
-        }
-      } else {
-#pragma unroll
-        for (int ib = 0; ib < CT; ++ib) {
-          const int i = 16 * ib + l16;
-          if (i < n && n0 + g4 < d)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o_at[i * a.out_stride + n0 + g4 + x] = from_float<T>(o[ib][x]);
-        }
+        store();
       }
       stored = ALIGNED && n == C && columns;
       if (PBUF == 1) arrive<63>();                 // P is free
