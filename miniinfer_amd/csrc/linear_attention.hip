@@ -504,7 +504,7 @@ struct ChunkShape {
   }
 };
 
-// What bounds it (that workload, 192 us at 3.5 TB/s): the matrix cores are busy for 30% of the time, the vector ALUs and
+// What bounds it (that workload, 186 us at 3.6 TB/s; the counters at 198): the matrix cores are busy for 30% of the time, the vector ALUs and
 // the LDS for about as long, memory for half of it.  With 8 waves on a compute unit, all that the registers (256) and the
 // LDS (128 KB) allow, the waits between a head's products are not covered: without loads and stores it takes 142 us,
 // without stores 25 less, without any one of the products 0 to 17 less.  Chunks of 32 tokens are slower with heads of 128
