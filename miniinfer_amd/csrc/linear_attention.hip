@@ -504,12 +504,12 @@ struct ChunkShape {
   }
 };
 
-// What bounds it (that workload, 186 us at 3.6 TB/s; the counters at 198): the matrix cores are busy for 30% of the time, the vector ALUs and
-// the LDS for about as long, memory for half of it.  With 8 waves on a compute unit, all that the registers (256) and the
-// LDS (128 KB) allow, the waits between a head's products are not covered: without loads and stores it takes 142 us,
-// without stores 25 less, without any one of the products 0 to 17 less.  Chunks of 32 tokens are slower with heads of 128
-// (258 us for the whole call, 234 with 64) and quicker with heads up to 64, where several workgroups share a compute unit
-// (8,192 tokens, 32 heads: 76 us, 114 with 64).
+// What bounds it (that workload, 186 us at 3.6 TB/s; the counters at 198): the matrix cores are busy for 30% of the time,
+// the vector ALUs and the LDS for about as long, memory for half of it.  With 8 waves on a compute unit, all that the
+// registers (256) and the LDS (128 KB) allow, the waits between a head's products are not covered: without loads and stores
+// it took 142 us, without stores 25 less, without any one of the products 0 to 17 less.  Chunks of 32 tokens are slower
+// with heads of 128 (258 us for the whole call, 234 with 64) and quicker with heads up to 64, where several workgroups
+// share a compute unit (8,192 tokens, 32 heads: 76 us, 114 with 64).
 //
 // STATES: only what a segment adds to its request's state (from zero), left in `work`; the last segment's is not needed.
 // ALIGNED: rows of q, k, v and out start at multiples of 16 bytes, and a chunk of a tensor spans less than 2^31 bytes.
