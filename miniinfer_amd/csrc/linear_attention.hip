@@ -583,6 +583,8 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       if (tid < C) left[C - 1 - tid] = p;
     }
     for (int i = C + tid; i < 2 * C; i += Shape::threads) left[i] = 0.f;
+    if (!STATES && CX == 1)          // (of chunks of 32 tokens nobody makes P's block that is all behind its queries)
+      for (int i = tid; i < PBUF * Shape::p_bytes / 16; i += Shape::threads) reinterpret_cast<u32x4*>(p_lds)[i] = u32x4{0, 0, 0, 0};
     __syncthreads();
   };
 
@@ -717,21 +719,21 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     fetch_kv(t + C, 1);
     fetch_q();
     tables();
-    // the weights a^(i-j) of the P that the wave makes, and a^(i+1) of its tokens, both with the scale
-    constexpr int PW = (CT * CX + WAVES - 1) / WAVES;
-    int reach[PW];                   // i - j of a lane's first element: those of the next ones are less
-    f32x4 weight[PW][2];
+    // The wave's block of P, of those that some product reads: 16 queries and 16 tokens in chunks of 32 (three blocks), else
+    // 16 and 32 (six).  Waves without columns take one first.
+    constexpr int P_WIDE = CX == 1 ? 1 : 2, BLOCKS = CX == 1 ? 3 : 2 * CT - 2;
+    static_assert(CX <= 2 && BLOCKS <= WAVES, "a block to a wave");
+    const int idle = max(0, WAVES - (d - slice * VS + 15) / 16), block = columns ? idle + wave : wave - (WAVES - idle);
+    const int p_row = CX == 1 ? 16 * min(block, 1) : 16 * (block < CT ? block : block - CT + 2);
+    const int p_col = CX == 1 ? 16 * (block / 2) : block < CT ? 0 : 32;
+    // its weights a^(i-j) and the a^(i+1) of the wave's queries, both with the scale
+    const int reach = p_row + l16 - (p_col + g4);          // i - j of a lane's first element: those of the next ones are less
+    f32x4 weight[P_WIDE];
     float reached[CT];
 #pragma unroll
-    for (int y = 0; y < PW; ++y) {
-      const int x = wave + y * WAVES;
-      reach[y] = 16 * (x % CT) + l16 - (x / CT * 32 + g4);
+    for (int w = 0; w < P_WIDE; ++w)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        weight[y][0][i] = power[min(max(reach[y] - i, 0), C)] * a.scale;
-        weight[y][1][i] = power[min(max(reach[y] - 16 - i, 0), C)] * a.scale;
-      }
-    }
+      for (int i = 0; i < 4; ++i) weight[w][i] = power[min(max(reach - 16 * w - i, 0), C)] * a.scale;
 #pragma unroll
     for (int ib = 0; ib < CT; ++ib) reached[ib] = power[16 * ib + l16 + 1] * a.scale;
     // the state's parts, held for all query heads of a chunk where there are registers for them
@@ -766,41 +768,35 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       const char* const qt = q_lds + qb * Shape::q_bytes;
       const char* const kt = k_lds + kv * Shape::q_bytes;
       char* const pt = p_lds + pb * Shape::p_bytes;
-      // ---- P^T: to a wave 16 queries and 32 tokens, or that again for the next waves' worth of them.  All waves wait for
-      // it, so it goes before the other wave's products (32,768 tokens 229 us, without that 233)
+      // ---- P^T.  All waves wait for it, so it goes before the other wave's products (32,768 tokens 229 us, without that 233)
       __builtin_amdgcn_s_setprio(1);
+      if (block < BLOCKS) {
+        f32x4 p[P_WIDE];
 #pragma unroll
-      for (int y = 0; y < PW; ++y) {
-        const int x = wave + y * WAVES, ib = x % CT, jx = x / CT;
-        if (x >= CT * CX || 2 * jx > ib) continue;             // (no product below reads these)
-        f32x4 p0 = {0.f, 0.f, 0.f, 0.f}, p1 = p0;
+        for (int w = 0; w < P_WIDE; ++w) p[w] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int x0 = 0; x0 < KX; x0 += KB) {
-          pair qf[KB], k0[KB], k1[KB];
+          pair qf[KB], kf[P_WIDE][KB];
 #pragma unroll
           for (int kx = 0; kx < KB; ++kx) {
-            qf[kx] = operand(qt, q_at, 16 * ib, x0 + kx);
-            k0[kx] = operand(kt, q_at, 32 * jx, x0 + kx);
-            k1[kx] = operand(kt, q_at, 32 * jx + 16, x0 + kx);
+            qf[kx] = operand(qt, q_at, p_row, x0 + kx);
+#pragma unroll
+            for (int w = 0; w < P_WIDE; ++w) kf[w][kx] = operand(kt, q_at, p_col + 16 * w, x0 + kx);
           }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int kx = 0; kx < KB; ++kx) {
-            mma(p0, k0[kx], qf[kx]);
-            mma(p1, k1[kx], qf[kx]);
-          }
+          for (int kx = 0; kx < KB; ++kx)
+#pragma unroll
+            for (int w = 0; w < P_WIDE; ++w) mma(p[w], kf[w][kx], qf[kx]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p0[i] = reach[y] >= i ? p0[i] * weight[y][0][i] : 0.f;
-          p1[i] = reach[y] >= 16 + i ? p1[i] * weight[y][1][i] : 0.f;
-        }
-        const Split<T, 2> s0(p0), s1(p1);
+        for (int w = 0; w < P_WIDE; ++w) {
 #pragma unroll
-        for (int z = 0; z < PARTS; ++z) {
-          char* at = pt + z * Shape::part_bytes;
-          *reinterpret_cast<half*>(at + Tile<T, C>::at(16 * ib + l16, 32 * jx + g4)) = s0.part[z];
-          *reinterpret_cast<half*>(at + Tile<T, C>::at(16 * ib + l16, 32 * jx + 16 + g4)) = s1.part[z];
+          for (int i = 0; i < 4; ++i) p[w][i] = reach >= 16 * w + i ? p[w][i] * weight[w][i] : 0.f;   // (0 * inf is not 0)
+          const Split<T, 2> parts(p[w]);
+#pragma unroll
+          for (int z = 0; z < PARTS; ++z)
+            *reinterpret_cast<half*>(pt + z * Shape::part_bytes + Tile<T, C>::at(p_row + l16, p_col + 16 * w + g4)) = parts.part[z];
         }
       }
       __builtin_amdgcn_s_setprio(0);
