@@ -232,6 +232,12 @@ __device__ __forceinline__ void mma(f32x4& acc, f32x8 a, f32x8 b) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
 }
+// ...over the first half of them, as far as that is less work
+__device__ __forceinline__ void mma_first(f32x4& acc, s16x8 a, s16x8 b) { mma(acc, a, b); }
+__device__ __forceinline__ void mma_first(f32x4& acc, f32x8 a, f32x8 b) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
+}
 __device__ __forceinline__ s16x4 to_half(f32x4 x) { return __builtin_bit_cast(s16x4, __builtin_convertvector(x, bf16x4)); }
 __device__ __forceinline__ f32x4 widen(s16x4 h) {
   const mi_u32x2 u = __builtin_bit_cast(mi_u32x2, h);
@@ -871,7 +877,10 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
 #pragma unroll
           for (int z = 0; z < PARTS; ++z)
 #pragma unroll
-            for (int ib = 2 * jx; ib < CT; ++ib) mma(o[ib], vt[jx], pf[ib][jx][z]);
+            for (int ib = 2 * jx; ib < CT; ++ib) {
+              if (ib == 2 * jx) mma_first(o[ib], vt[jx], pf[ib][jx][z]);     // (the other half is behind the queries)
+              else mma(o[ib], vt[jx], pf[ib][jx][z]);
+            }
         store();
       } else {
         // a masked weight of zero times a value that is not finite would reach the tokens before it: only what a token
