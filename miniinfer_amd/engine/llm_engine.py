@@ -160,7 +160,8 @@ class LLMEngine:
     product kernels are timed at start-up, that timing's buffers instead if they are larger.  The 32-bit logits of
     `max_num_seqs` rows with the sampler's scratch.  The captured decode steps: they share one pool for what they
     hold while they run (counted once, for the widest of them) but each keeps its own logits, so one row of logits for
-    every row of every (batch, table width) bucket that this engine's limits allow.  And 256 MiB of slack (key-range
+    every row of every (batch, table width) bucket that this engine's limits allow.  What the parts' own kernels need
+    beside activations (`Part.workspace_bytes`).  And 256 MiB of slack (key-range
     partials of the attention, the k-split products' partial results, the library's workspace)."""
     cfg, spec = self.config, self.model.spec
     esize = 2 if self.dtype == torch.bfloat16 else 4
@@ -181,7 +182,8 @@ class LLMEngine:
       from .runner import graph_bucket_rows
       rows, widths = graph_bucket_rows(cfg.max_num_seqs, self.max_model_len, cfg.page_size)
       graphs = 256 * per_token + rows * widths * 4 * spec.vocab_size
-    return int(step + logits + graphs + (256 << 20))
+    workspace = getattr(self.model, "largest_workspace_bytes", lambda *a: 0)(T, min(cfg.max_num_seqs, T))
+    return int(step + logits + graphs + workspace + (256 << 20))
 
   @staticmethod
   def _eos_of_folder(path: str):

@@ -1196,6 +1196,19 @@ def _linear_attention_call(what, q, k, v, nq, nkv, d, out, state, state_rows, cu
           nq, nkv, d, log_decay.data_ptr(), scale)
 
 
+def _linear_attention_workgroups(nkv: int, d: int, itemsize: int, units: int) -> int:
+  """Workgroups of a head that run at once."""
+  columns = 64 if d <= 64 or (itemsize == 4 and d > 128) else 128      # of a workgroup
+  return units * (2 if d <= 64 else 1) // (nkv * -(-d // columns))
+
+
+def linear_attention_workspace(num_tokens: int, num_requests: int, nkv: int, d: int, itemsize: int = 2, units: int = 256) -> int:
+  """The most bytes that `linear_attention` allocates beside its output for up to so many tokens and requests: a state
+  for each segment."""
+  segments = min(num_tokens // 64, max(1, _linear_attention_workgroups(nkv, d, itemsize, units)))
+  return 4 * (segments + num_requests) * nkv * d * d if num_tokens > 2 * 64 else 0
+
+
 def linear_attention_segment(num_tokens: int, num_requests: int, max_len: int, nkv: int, d: int, itemsize: int = 2,
                              units: int = 256) -> int:
   """Tokens of a segment into which requests are cut, 0 for none: as many (whole chunks of 64) as make one workgroup for
@@ -1204,8 +1217,7 @@ def linear_attention_segment(num_tokens: int, num_requests: int, max_len: int, n
   requests of 8,192 tokens together, 8 heads of 128: 67 us in segments of 384, 89 in segments of 256).  A cut costs a pass
   over the keys and values for the segments' states and a kernel that adds them up, so a longest request of up to two
   segments is left whole (24 requests of up to 950 tokens, 12 heads of 80: 74 us whole, 93 in segments of 384)."""
-  columns = 64 if d <= 64 or (itemsize == 4 and d > 128) else 128      # of a workgroup
-  workgroups = units * (2 if d <= 64 else 1) // (nkv * -(-d // columns))
+  workgroups = _linear_attention_workgroups(nkv, d, itemsize, units)
   tokens = max(64, -(-num_tokens // (64 * max(1, workgroups - num_requests + 1, workgroups // 2))) * 64)
   return tokens if max_len > 2 * tokens else 0
 

@@ -116,6 +116,15 @@ class Part:
       out.update(child.all_kernel_modules())
     return sorted(out)
 
+  def workspace_bytes(self, tokens: int, requests: int) -> int:
+    """Device memory that the part's kernels hold beside activations in a step of so many tokens and requests, at most."""
+    return 0
+
+  def largest_workspace_bytes(self, tokens: int, requests: int) -> int:
+    """The most that any one part below needs: they run one after another."""
+    return max([self.workspace_bytes(tokens, requests)]
+               + [child.largest_workspace_bytes(tokens, requests) for _, child in self.children()])
+
   def is_capturable(self) -> bool:
     return bool(self.capturable) and all(child.is_capturable() for _, child in self.children())
 

@@ -27,6 +27,10 @@ class LinearAttention(PagedAttention):
   def cache_requirement(self):
     return FixedState(shape=(self.nkv, self.d, self.d), dtype=torch.float32)
 
+  def workspace_bytes(self, tokens: int, requests: int) -> int:
+    itemsize = 2 if self.ctx.dtype == torch.bfloat16 else 4
+    return ops.linear_attention_workspace(tokens, requests, self.nkv, self.d, itemsize, ops.compute_units())
+
   def _rotate(self, qkv: torch.Tensor, ctx) -> None:
     """Head norms and rotation of q and k, in place."""
     nq, nkv, d = self.nq, self.nkv, self.d

@@ -67,3 +67,31 @@ def test_segments_of_several_chunks(dtype, nq, nkv, d, segment, monkeypatch):
   c.check(out, state)
   again = c.run()
   assert torch.equal(out, again[0]) and torch.equal(state, again[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_call_allocates_no_more_than_is_stated(dtype):
+  from miniinfer_amd.kernels import ops
+  for nq, nkv, d, lens in ((2, 1, 128, [2500]), (8, 8, 64, [900, 300]), (2, 2, 256, [700, 700, 5])):
+    c = _Call(dtype, nq, nkv, d, lens, seed=9)
+    qkv, state, rows, cu, g = c.device()
+    out = torch.empty(c.T, nq * d, dtype=dtype, device=DEV)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.linear_attention(*c.parts(qkv), nq, nkv, d, out, state, rows, cu, g, c.scale)
+    room = ops.linear_attention_workspace(c.T, len(lens), nkv, d, out.element_size(), ops.compute_units())
+    assert 0 < torch.cuda.max_memory_allocated() - before <= room + 512          # (the allocator's grain)
+
+
+def test_the_engine_leaves_room_for_it(tmp_path):
+  from miniinfer_amd import LLMEngine
+  from miniinfer_amd.kernels import ops
+  from test_linear_attention_model_gpu import _write
+  _write(str(tmp_path / "m"), "bfloat16")
+  with LLMEngine(model=str(tmp_path / "m"), dtype="bfloat16", page_size=16, num_pages=40, max_num_seqs=8,
+                 tune_products=False) as eng:
+    counted = eng.activation_bytes()
+    stated = eng.model.largest_workspace_bytes(eng.config.max_num_batched_tokens, 8)
+    eng.model.largest_workspace_bytes = lambda *a: 0
+    assert stated > 0 and counted - eng.activation_bytes() == stated

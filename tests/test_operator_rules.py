@@ -85,3 +85,33 @@ def test_a_search_has_candidates_for_every_beam_whatever_ends(eos, stop, ignore,
   assert new(most).count >= most * (1 + len(set(stop) | (set() if ignore else set(eos))))
   with pytest.raises(ValueError, match="at most"):
     new(most + 1)
+
+
+@pytest.mark.parametrize("nkv,d,itemsize", [(1, 8, 2), (12, 64, 4), (32, 64, 2), (8, 128, 2), (12, 80, 2), (4, 256, 4), (700, 128, 2)])
+def test_the_stated_workspace_holds_every_call(nkv, d, itemsize):
+  """For all token and request counts up to those it is stated for."""
+  for most_tokens in (1, 128, 129, 1000, 8192, 40000):
+    for most_requests in (1, 5, 64, 256):
+      room = ops.linear_attention_workspace(most_tokens, most_requests, nkv, d, itemsize)
+      for tokens in {most_tokens, most_tokens // 2, most_tokens // 3, min(most_tokens, 200)}:
+        for requests in {1, most_requests, max(1, most_requests // 2)}:
+          segment = ops.linear_attention_segment(tokens, requests, tokens, nkv, d, itemsize)
+          if segment:
+            assert 4 * (tokens // segment + requests) * nkv * d * d <= room
+
+
+def test_parts_state_their_workspaces():
+  from miniinfer_amd.parts import Part
+
+  class Child(Part):
+    def __init__(self, each):
+      self.each = each
+
+    def workspace_bytes(self, tokens, requests):
+      return self.each * tokens + requests
+
+  class Parent(Part):
+    def children(self):
+      return [("a", Child(3)), ("b", Child(5))]
+
+  assert Parent().largest_workspace_bytes(7, 2) == 37 and Part().largest_workspace_bytes(7, 2) == 0
