@@ -185,9 +185,10 @@ MI_EXPORT int mi_linear_attention_step(LA_ARGS, hipStream_t stream) {
 //   O^T += V^T P^T     V^T by the LDS's transposing reads
 //   S  += K^T (w V)    K^T likewise
 //
-// Roundings of the bfloat16 form: what is 32-bit (S, the weighted P and w V) is split into bfloat16 parts that are
-// multiplied one after the other into the same accumulators: two parts (what is left out is 2^-17 of a term) for what
-// ends in a bfloat16 output, three (2^-25) for the state, which is 32-bit whatever the inputs are.
+// The bfloat16 form multiplies what is 32-bit (S, the weighted P and w V) as it is: split into three bfloat16 parts whose sum
+// it is to the last bit, one after the other into the same accumulators.  (Two parts for S and P leave out 2^-17 of a term,
+// which an output keeps where its terms cancel; they were 8 to 11% quicker, 32,768 tokens 227 us against 252.)  The one
+// rounding to fewer bits is the output's.
 //
 // Operands: lane l of an operand has row l % 16 and, of 32 elements of the summed axis, with g = l / 16: in bfloat16
 // (16x16x32) the 8 from 8 g on, in 32 bits (eight products 16x16x4) the 4 from 4 g on and the 4 from 16 + 4 g on.  Its
@@ -246,26 +247,33 @@ __device__ __forceinline__ f32x4 widen(s16x4 h) {
 }
 __device__ __forceinline__ f32x4 widen(f32x4 h) { return h; }
 
-// A 32-bit value as a sum of parts that the matrix cores take.
-template <typename T, int PARTS>
+// A 32-bit value as a sum of parts that the matrix cores take, exactly: a part is what is left cut off after 8 bits, and
+// 24 bits are three times 8.
+template <typename T>
 struct Split;
-template <int PARTS>
-struct Split<bf16, PARTS> {
-  s16x4 part[PARTS];
+template <>
+struct Split<bf16> {
+  static constexpr int parts = 3;
+  s16x4 part[parts];
+  static __device__ __forceinline__ s16x4 first(f32x4 x) {
+    auto two = [&](int i) { return __builtin_amdgcn_perm(__float_as_uint(x[i + 1]), __float_as_uint(x[i]), 0x07060302); };
+    return __builtin_bit_cast(s16x4, mi_u32x2{two(0), two(2)});
+  }
   __device__ __forceinline__ explicit Split(f32x4 x) {
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
-      part[p] = to_half(x);
-      if (p + 1 < PARTS) x -= widen(part[p]);
+    for (int p = 0; p < parts; ++p) {
+      part[p] = first(x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] -= __uint_as_float(__float_as_uint(x[i]) & 0xffff0000u);
     }
   }
-  static constexpr int parts = PARTS;
 };
-template <int PARTS>
-struct Split<float, PARTS> {
-  f32x4 part[1];
-  __device__ __forceinline__ explicit Split(f32x4 x) : part{x} {}
+template <>
+struct Split<float> {
   static constexpr int parts = 1;
+  f32x4 part[1];
+  static __device__ __forceinline__ f32x4 first(f32x4 x) { return x; }
+  __device__ __forceinline__ explicit Split(f32x4 x) : part{x} {}
 };
 
 // A tile of whole rows in LDS: piece p of row r lies at place p ^ swap(r) of it.
@@ -502,7 +510,7 @@ template <typename T, int DP, int WAVES, int C, int PBUF>
 struct ChunkShape {
   static constexpr int waves = WAVES, threads = 64 * WAVES;
   static constexpr int VS = 16 * waves;
-  static constexpr int parts = sizeof(T) == 2 ? 2 : 1;
+  static constexpr int parts = Split<T>::parts;
   static constexpr int q_bytes = C * Tile<T, DP>::stride, v_bytes = C * Tile<T, VS>::stride;
   static constexpr int part_bytes = C * Tile<T, C>::stride, p_bytes = parts * part_bytes;
   static constexpr int lds(bool states) {
@@ -662,13 +670,13 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       for (int y = 0; y < 2; ++y)
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[y][i] = left[C - n + summed<T>(j, y, g, i)];
-      const Split<T, 3> v0(half_of(vt[j], 0) * w[0]), v1(half_of(vt[j], 1) * w[1]);
+      const Split<T> v0(half_of(vt[j], 0) * w[0]), v1(half_of(vt[j], 1) * w[1]);
 #pragma unroll
       for (int x0 = 0; x0 < KX; x0 += 2) {
         pair kd[2][2];
         dims_down(kd, kb, k_down, j, x0);
 #pragma unroll
-        for (int z = 0; z < Split<T, 3>::parts; ++z)
+        for (int z = 0; z < Split<T>::parts; ++z)
 #pragma unroll
           for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -735,15 +743,13 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     // its weights a^(i-j) and the a^(i+1) of the wave's queries, both with the scale
     const int reach = p_row + l16 - (p_col + g4);          // i - j of a lane's first element: those of the next ones are less
     f32x4 weight[P_WIDE];
-    float reached[CT];
 #pragma unroll
     for (int w = 0; w < P_WIDE; ++w)
 #pragma unroll
       for (int i = 0; i < 4; ++i) weight[w][i] = power[min(max(reach - 16 * w - i, 0), C)] * a.scale;
-#pragma unroll
-    for (int ib = 0; ib < CT; ++ib) reached[ib] = power[16 * ib + l16 + 1] * a.scale;
-    // the state's parts, held for all query heads of a chunk where there are registers for them
-    constexpr bool HELD = DP <= 128;
+    // the state's parts but the first, which is the state's upper halves: held for all query heads of a chunk where there
+    // are registers for them
+    constexpr bool HELD = DP <= 128 && PARTS > 1;
     pair sp[HELD ? KX : 1][PARTS];
     bool odd = false;                // whether one of the wave's values is not finite
     bool stored = false;             // whether the last head's rows of out are known to be STORES stores of the wave
@@ -765,9 +771,9 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
         if (HELD) {
 #pragma unroll
           for (int x = 0; x < KX; ++x) {
-            const Split<T, 2> s0(s[x][0]), s1(s[x][1]);
+            const Split<T> s0(s[x][0]), s1(s[x][1]);
 #pragma unroll
-            for (int z = 0; z < PARTS; ++z) sp[x][z] = join(s0.part[z], s1.part[z]);
+            for (int z = 1; z < PARTS; ++z) sp[x][z] = join(s0.part[z], s1.part[z]);
           }
         }
       }
@@ -799,7 +805,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
         for (int w = 0; w < P_WIDE; ++w) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[w][i] = reach >= 16 * w + i ? p[w][i] * weight[w][i] : 0.f;   // (0 * inf is not 0)
-          const Split<T, 2> parts(p[w]);
+          const Split<T> parts(p[w]);
 #pragma unroll
           for (int z = 0; z < PARTS; ++z)
             *reinterpret_cast<half*>(pt + z * Shape::part_bytes + Tile<T, C>::at(p_row + l16, p_col + 16 * w + g4)) = parts.part[z];
@@ -822,17 +828,18 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
           }
           __builtin_amdgcn_sched_barrier(0);
           if (!HELD) {
-            const Split<T, 2> s0(s[x][0]), s1(s[x][1]);
+            const Split<T> s0(s[x][0]), s1(s[x][1]);
 #pragma unroll
-            for (int z = 0; z < PARTS; ++z) sp[0][z] = join(s0.part[z], s1.part[z]);
+            for (int z = 1; z < PARTS; ++z) sp[0][z] = join(s0.part[z], s1.part[z]);
           }
+          sp[HELD ? x : 0][0] = join(Split<T>::first(s[x][0]), Split<T>::first(s[x][1]));
 #pragma unroll
           for (int z = 0; z < PARTS; ++z)
 #pragma unroll
             for (int ib = 0; ib < CT; ++ib) mma(o[ib], sp[HELD ? x : 0][z], qf[x & 1][ib]);
         }
 #pragma unroll
-        for (int ib = 0; ib < CT; ++ib) o[ib] *= reached[ib];
+        for (int ib = 0; ib < CT; ++ib) o[ib] *= power[16 * ib + l16 + 1] * a.scale;
         if (last && (t + n < hi || s_to)) update(kv, n);
       }
       // P is whole; the next head's Q and, after the last head, the next chunk's K and V are here: all that was asked for
@@ -864,23 +871,26 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       // ---- what the chunk's own tokens give
       if (!columns) {
       } else if (!odd) {
-        pair pf[CT][CX][PARTS];
+        pair pf[2][CT][CX];            // of a part of P; the next part's reads go before this one's products
+        auto read_p = [&](int z) {
 #pragma unroll
-        for (int ib = 0; ib < CT; ++ib)
+          for (int ib = 0; ib < CT; ++ib)
 #pragma unroll
-          for (int jx = 0; 2 * jx <= ib; ++jx)
+            for (int jx = 0; 2 * jx <= ib; ++jx) pf[z & 1][ib][jx] = operand(pt + z * Shape::part_bytes, p_at, 16 * ib, jx);
+        };
+        read_p(0);
 #pragma unroll
-            for (int z = 0; z < PARTS; ++z) pf[ib][jx][z] = operand(pt + z * Shape::part_bytes, p_at, 16 * ib, jx);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int z = 0; z < PARTS; ++z) {
+          if (z + 1 < PARTS) read_p(z + 1);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int jx = 0; jx < CX; ++jx)
-#pragma unroll
-          for (int z = 0; z < PARTS; ++z)
+          for (int jx = 0; jx < CX; ++jx)
 #pragma unroll
             for (int ib = 2 * jx; ib < CT; ++ib) {
-              if (ib == 2 * jx) mma_first(o[ib], vt[jx], pf[ib][jx][z]);     // (the other half is behind the queries)
-              else mma(o[ib], vt[jx], pf[ib][jx][z]);
+              if (ib == 2 * jx) mma_first(o[ib], vt[jx], pf[z & 1][ib][jx]);     // (the other half is behind the queries)
+              else mma(o[ib], vt[jx], pf[z & 1][ib][jx]);
             }
+        }
         store();
       } else {
         // a masked weight of zero times a value that is not finite would reach the tokens before it: only what a token
