@@ -1202,11 +1202,16 @@ def _linear_attention_workgroups(nkv: int, d: int, itemsize: int, units: int) ->
   return units * (2 if d <= 64 else 1) // (nkv * -(-d // columns))
 
 
+# What a block of the caching allocator may hold beyond what was asked for: it hands out a free block whole when the rest
+# would be 1 MiB or less, and rounds sizes to 512 bytes.
+ALLOCATOR_REST = (1 << 20) + 512
+
+
 def linear_attention_workspace(num_tokens: int, num_requests: int, nkv: int, d: int, itemsize: int = 2, units: int = 256) -> int:
-  """The most bytes that `linear_attention` allocates beside its output for up to so many tokens and requests: a state
-  for each segment."""
+  """The most bytes that a call of `linear_attention` takes beside its output for up to so many tokens and requests: a state
+  for each segment, in one block of the caching allocator, with the rest that such a block may have."""
   segments = min(num_tokens // 64, max(1, _linear_attention_workgroups(nkv, d, itemsize, units)))
-  return 4 * (segments + num_requests) * nkv * d * d if num_tokens > 2 * 64 else 0
+  return 4 * (segments + num_requests) * nkv * d * d + ALLOCATOR_REST if num_tokens > 2 * 64 else 0
 
 
 def linear_attention_segment(num_tokens: int, num_requests: int, max_len: int, nkv: int, d: int, itemsize: int = 2,
