@@ -18,6 +18,7 @@ request gives everything back (kv_cache_manager.py:718-750).
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 from typing import Dict, Hashable, List, Optional, Sequence, Tuple
 
@@ -218,8 +219,9 @@ class CacheManager:
   @classmethod
   def storage_bytes(cls, layer_needs: Sequence[object], page_size: int, num_pages: int, max_requests: int,
                     max_step_tokens: int, dtype: torch.dtype) -> int:
-    """Device bytes of the page pools for `num_pages` (scratch pages included)."""
-    total = 0
+    """Device bytes of the page pools for `num_pages` (scratch pages included) and of the fixed-size states of
+    `max_requests` requests (with the scratch row)."""
+    total = cls.state_bytes(layer_needs, max_requests, dtype)
     for n in layer_needs:
       if isinstance(n, PagedKV):
         P = n.page_size or page_size
@@ -227,6 +229,12 @@ class CacheManager:
         pages = cls.group_pages(n, page_size, num_pages, max_requests, max_step_tokens) + 1
         total += 2 * n.num_kv_heads * n.head_dim * P * esize * pages
     return total
+
+  @staticmethod
+  def state_bytes(layer_needs: Sequence[object], max_requests: int, dtype: torch.dtype) -> int:
+    """Device bytes of the fixed-size states, however many pages there are."""
+    return sum((max_requests + 1) * math.prod(n.shape) * torch.empty((), dtype=n.dtype or dtype).element_size()
+               for n in layer_needs if isinstance(n, FixedState))
 
   @staticmethod
   def bytes_per_page(layer_needs: Sequence[object], page_size: int, dtype: torch.dtype) -> int:

@@ -129,7 +129,8 @@ class LLMEngine:
     holds back a fifth of the free memory for them, whatever the model: utils/memory_utils.py:85-144; here the
     step's buffers are counted from the model's sizes and the token budget).  Never more pages than
     `max_num_seqs` requests of `max_model_len` tokens can use.  The pools' bytes are the cache manager's own count
-    (groups differ in page size, dtype and, with a window, in how many pages they can use at all)."""
+    (groups differ in page size, dtype and, with a window, in how many pages they can use at all), the fixed-size states
+    of `max_num_seqs` requests among them, which do not depend on the pages."""
     cfg = self.config
     cap = cfg.max_num_seqs * (-(-self.max_model_len // cfg.page_size))
 
@@ -137,13 +138,17 @@ class LLMEngine:
       return CacheManager.storage_bytes(needs, cfg.page_size, pages, cfg.max_num_seqs, cfg.max_num_batched_tokens,
                                         self.dtype)
 
+    states = CacheManager.state_bytes(needs, cfg.max_num_seqs, self.dtype)
     if pool_bytes(cap) == 0:
       return max(1, cap)
     free, total = torch.cuda.mem_get_info(self.device)
     usable = free - int(total * (1.0 - cfg.gpu_memory_utilization)) - self.activation_bytes()
     if pool_bytes(2) > usable:
       raise RuntimeError(f"not enough device memory for a cache: {free >> 20} MiB free, the largest step needs "
-                         f"{self.activation_bytes() >> 20} MiB, two pages cost {pool_bytes(2)} bytes")
+                         f"{self.activation_bytes() >> 20} MiB, the fixed-size states of {cfg.max_num_seqs} requests "
+                         f"{states >> 20} MiB, two pages cost {pool_bytes(2) - states} bytes")
+    if pool_bytes(cap) == states:        # no layer is paged
+      return max(1, cap)
     lo, hi = 2, cap                      # the most pages whose pools fit: the bytes grow with the pages
     while lo < hi:
       mid = (lo + hi + 1) // 2
