@@ -82,21 +82,30 @@ class BeamSearcher:
     self.next_request += 1
     return ("beam", self.next_request)
 
-  def _pages(self, search: Search) -> List[int]:
-    """The most pages a search holds at once, per cache group: its prompt's, shared, and for each beam those of its own
-    tokens, with the page that the prompt ends in and the one that a fork starts on."""
+  def _pages(self, searches: Sequence[Search]) -> List[int]:
+    """The most pages that searches side by side hold at once, per cache group: their prompts', shared, and for each beam
+    those of its own tokens, with the page that the prompt ends in and the one that a fork starts on.  Of a group with a
+    window a request keeps what its next token can see, at most ceil(window / page) + 1 pages, and in a step the new
+    tokens' beside them: one page of a beam, while the prompts are read those of a step's tokens."""
     out = []
     for g in self.cache.paged:
-      P = g.page_size
-      out.append(-(-len(search.prompt) // P) + self.params.num_beams * (-(-search.max_tokens // P) + 2))
+      pages = lambda n: -(-n // g.page_size)
+      prompts = [pages(len(s.prompt)) for s in searches]
+      own = [self.params.num_beams * (pages(s.max_tokens) + 2) for s in searches]
+      if g.need.window is None:
+        out.append(sum(prompts) + sum(own))
+        continue
+      keeps = pages(g.need.window) + 1
+      reading = min(sum(prompts), sum(min(p, keeps + 1) for p in prompts) + pages(self.engine.config.max_num_batched_tokens))
+      searching = sum(min(min(p, keeps) + o, self.params.num_beams * (keeps + 1)) for p, o in zip(prompts, own))
+      out.append(max(reading, searching))
     return out
 
   def _fits(self, searches: Sequence[Search]) -> bool:
     beams = len(searches) * self.params.num_beams          # the tokens of a step
     if beams > self.cache.num_free_slots() or beams > self.engine.config.max_num_batched_tokens:
       return False
-    needs = [self._pages(s) for s in searches]
-    return all(sum(n[gi] for n in needs) <= room for gi, room in enumerate(self.cache.room()))
+    return all(need <= room for need, room in zip(self._pages(searches), self.cache.room()))
 
   # ------------------------------------------------------------------ steps
   def _prefill(self, searches: Sequence[Search]) -> torch.Tensor:
@@ -177,7 +186,7 @@ class BeamSearcher:
     for s in searches:
       if not self._fits([s]):
         raise ValueError(f"a beam search of {self.params.num_beams} beams over a prompt of {len(s.prompt)} tokens plus "
-                         f"max_tokens={s.max_tokens} does not fit the cache ({self._pages(s)} pages per group, "
+                         f"max_tokens={s.max_tokens} does not fit the cache ({self._pages([s])} pages per group, "
                          f"{self.cache.room()} free; {self.cache.num_free_slots()} request slots; steps of "
                          f"{self.engine.config.max_num_batched_tokens} tokens)")
     try:
