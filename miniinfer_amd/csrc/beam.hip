@@ -11,7 +11,7 @@
 // Candidates of different beams lie closer to one another than a 32-bit score can tell apart (32 bits of a score of
 // -40 are steps of 4e-6, and a hundred thousand candidates share a few units), so exponentials, sums and compared scores
 // are 64-bit; the exponential is a polynomial good to 3e-12, half of the arithmetic of the pass, and hides behind the
-// loads.
+// loads.  The running scores come and go in 32 or 64 bits: a search that keeps them in 64 keeps that order from step to step.
 #include "common.h"
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -398,11 +398,11 @@ __global__ __launch_bounds__(BEAM_THREADS, 4) void beam_rows_kernel(const float*
   }
 }
 
-// Block: a group.
-template <int WAVES>
+// Block: a group.  S: the type of the running scores.
+template <int WAVES, typename S>
 __global__ __launch_bounds__(WAVES * MI_WAVE) void beam_pick_kernel(const float* __restrict__ logits, int64_t row_stride,
-                                                                 const float* __restrict__ scores, BeamParts in, int beams,
-                                                                 int count, int parts, int V, float* __restrict__ out_scores,
+                                                                 const S* __restrict__ scores, BeamParts in, int beams,
+                                                                 int count, int parts, int V, S* __restrict__ out_scores,
                                                                  int* __restrict__ out_beams, int* __restrict__ out_tokens) {
   __shared__ float row_max[BEAM_MAX_BEAMS];
   __shared__ double row_base[BEAM_MAX_BEAMS];      // scores[b] - log of the row's sum; NaN: no candidate above -inf
@@ -434,10 +434,10 @@ __global__ __launch_bounds__(WAVES * MI_WAVE) void beam_pick_kernel(const float*
 #pragma unroll
     for (int step = 1; step < 16; step <<= 1) s += xor_lane(s, step, lane);
     if (b < beams && l == 0) {
-      const float start = scores[r0 + b];
-      const bool dead = !(fabsf(start) < INFINITY) || m == -INFINITY;
+      const double start = (double)scores[r0 + b];
+      const bool dead = !(fabs(start) < INFINITY) || m == -INFINITY;
       row_max[b] = m;
-      row_base[b] = dead ? NAN : (double)start - log(s);
+      row_base[b] = dead ? NAN : start - log(s);
       if (dead || m == INFINITY) special = 1;
     }
   }
@@ -473,7 +473,7 @@ __global__ __launch_bounds__(WAVES * MI_WAVE) void beam_pick_kernel(const float*
     const int place = joined_place(xs, is, WAVES, count, i / count, i % count);
     if (place < count) {
       const int64_t to = (int64_t)blockIdx.x * count + place;
-      out_scores[to] = (float)xs[i];
+      out_scores[to] = (S)xs[i];
       out_beams[to] = is[i] / V;
       out_tokens[to] = is[i] % V;
     }
@@ -498,8 +498,9 @@ MI_EXPORT int64_t mi_beam_scratch(int groups, int beams, int V, int count, int u
   return rows * parts * (2 + count);
 }
 
-MI_EXPORT int mi_beam_select(const float* logits, int64_t row_stride, const float* scores, int groups, int beams, int V,
-                             int count, int units, double* scratch, float* out_scores, int* out_beams, int* out_tokens,
+// wide: scores and out_scores are double, else float.
+MI_EXPORT int mi_beam_select(const float* logits, int64_t row_stride, const void* scores, int groups, int beams, int V,
+                             int count, int units, int wide, double* scratch, void* out_scores, int* out_beams, int* out_tokens,
                              hipStream_t stream) {
   MI_REQUIRE(groups >= 0 && beams >= 1 && V >= 1 && row_stride >= V && units >= 1, "beam_select: bad sizes groups=%d beams=%d V=%d stride=%lld",
              groups, beams, V, (long long)row_stride);
@@ -518,12 +519,15 @@ MI_EXPORT int mi_beam_select(const float* logits, int64_t row_stride, const floa
   p.token = (int*)(p.x + rows * parts * count);
   beam_rows_kernel<<<(uint32_t)(rows * parts), BEAM_THREADS, 0, stream>>>(logits, row_stride, V, count, parts, tiles, p);
   MI_CHECK_LAUNCH("beam rows");
-  if (beams * parts * count > BEAM_FEW)
-    beam_pick_kernel<16><<<groups, 16 * MI_WAVE, 0, stream>>>(logits, row_stride, scores, p, beams, count, parts, V, out_scores,
-                                                              out_beams, out_tokens);
-  else
-    beam_pick_kernel<4><<<groups, 4 * MI_WAVE, 0, stream>>>(logits, row_stride, scores, p, beams, count, parts, V, out_scores,
-                                                            out_beams, out_tokens);
+  const bool many = beams * parts * count > BEAM_FEW;
+#define PICK(WAVES, S)                                                                                                  \
+  beam_pick_kernel<WAVES, S><<<groups, WAVES * MI_WAVE, 0, stream>>>(logits, row_stride, (const S*)scores, p, beams, count, parts, V, \
+                                                                     (S*)out_scores, out_beams, out_tokens)
+  if (many && wide) PICK(16, double);
+  else if (many) PICK(16, float);
+  else if (wide) PICK(4, double);
+  else PICK(4, float);
+#undef PICK
   MI_CHECK_LAUNCH("beam pick");
   return 0;
 }

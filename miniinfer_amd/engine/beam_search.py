@@ -22,7 +22,7 @@ from .runner import StepEntry
 class Beam:
   req: Tuple                    # its request in the cache
   tokens: List[int]             # generated so far
-  score: float                  # sum of their log-probabilities
+  score: float                  # sum of their log-probabilities, in 64 bits as they are compared
 
 
 @dataclass
@@ -141,7 +141,8 @@ class BeamSearcher:
     for s in searches:
       scores += [b.score for b in s.beams] + [float("-inf")] * (width - len(s.beams))
     count = min(self.count, width * V)
-    got = ops.beam_select(logits, torch.tensor(scores, dtype=torch.float32).to(logits.device), width, count)
+    got = ops.beam_select(logits, torch.tensor(scores, dtype=torch.float64).to(logits.device), width, count,
+                          score_dtype=torch.float64)
     values, beams, tokens = (t.tolist() for t in got)
     forks: List[Tuple] = []
     for s, vs, bs, ts in zip(searches, values, beams, tokens):

@@ -177,7 +177,7 @@ _SIGS["linear_attention"] = {
 }
 
 _SIGS["beam"] = {
-  "mi_beam_select": [c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+  "mi_beam_select": [c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                      c_void_p],
   "mi_beam_scratch": [c_int, c_int, c_int, c_int, c_int],
 }
@@ -1280,15 +1280,17 @@ BEAM_MAX_COUNT = 64
 BEAM_MAX_BEAMS = 64
 
 
-def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_beams: int,
-                count: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_beams: int, count: int,
+                score_dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
   """The `count` best continuations of every group of `num_beams` beams: of
 
       scores[b] + logits[b, v] - log sum_u exp(logits[b, u])      b over the group's beams, v over the vocabulary
 
   the largest, largest first, equal ones by (beam, token).  logits float32 [G * num_beams, V] with dense rows, scores
-  float32 [G * num_beams] (-inf, or anything else that is not finite: a beam that does not take part).  Returns (scores
-  float32, beams int32 in 0 .. num_beams - 1, tokens int32), each [G, count].  A logit that is NaN counts as -inf; where a row holds +inf, those
+  [G * num_beams] (-inf, or anything else that is not finite: a beam that does not take part).  Returns (scores, beams
+  int32 in 0 .. num_beams - 1, tokens int32), each [G, count].  score_dtype: of the scores given and returned, float32 or
+  float64 (scores that a search adds up over its steps: in 32 bits, steps of 4e-6 at -40, each step's rounding would
+  decide between beams that the next one cannot tell apart).  A logit that is NaN counts as -inf; where a row holds +inf, those
   tokens share its mass; a row of -inf only has no candidate above -inf.  If fewer than `count` candidates are above -inf
   the rest of the list has score -inf.  Sums of exponentials and the scores that are compared are 64-bit."""
   if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
@@ -1298,7 +1300,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_beams: int,
     raise KernelError(f"beam_select: logits {tuple(logits.shape)} are no groups of {num_beams} beams")
   if R > 1 and logits.stride(0) < V:
     raise KernelError("beam_select: rows of logits overlap")
-  _f32("scores", scores, R)
+  if score_dtype is torch.float64:
+    if scores.dtype is not torch.float64 or not scores.is_contiguous() or scores.numel() != R:
+      raise KernelError(f"beam_select: scores must be contiguous float64 [{R}], got {scores.dtype} {tuple(scores.shape)}")
+  elif score_dtype is torch.float32:
+    _f32("scores", scores, R)
+  else:
+    raise KernelError(f"beam_select: scores are float32 or float64, not {score_dtype}")
   G = R // num_beams
   if num_beams * V >= 1 << 31:
     raise KernelError(f"beam_select: {num_beams} beams x {V} tokens are too many")
@@ -1309,10 +1317,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_beams: int,
     lib = _lib("beam")
     units = compute_units(logits.get_device())
     scratch = torch.empty(lib.mi_beam_scratch(G, num_beams, V, count, units), dtype=torch.float64, device=logits.device)
-    out_scores = torch.empty((G, count), dtype=torch.float32, device=logits.device)
+    out_scores = torch.empty((G, count), dtype=score_dtype, device=logits.device)
     beams, tokens = torch.empty((2, G, count), dtype=torch.int32, device=logits.device).unbind()
     _check(lib, lib.mi_beam_select(logits.data_ptr(), logits.stride(0) if R > 1 else V, scores.data_ptr(), G, num_beams, V, count,
-                                   units, scratch.data_ptr(), out_scores.data_ptr(), beams.data_ptr(), tokens.data_ptr(), stream))
+                                   units, int(score_dtype is torch.float64), scratch.data_ptr(), out_scores.data_ptr(), beams.data_ptr(), tokens.data_ptr(), stream))
   return out_scores, beams, tokens
 
 
