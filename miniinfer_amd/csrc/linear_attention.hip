@@ -15,8 +15,11 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 #define LA_MAX_D 256
 
 // a^n; a^0 = 1 for a decay of zero too.  (The product's rounding puts an error of |n log a| 2^-24 on the power, at most
-// 0.4 * 2^-24 of the weight 1 for a decay.)
-__device__ __forceinline__ float decay_power(float log_decay, int n) { return n == 0 ? 1.f : expf(log_decay * n); }
+// 0.4 * 2^-24 of the weight 1 for a decay.)  Only a decay of zero has powers of zero, the others end at the
+// smallest normal number: an infinity in a state or a value does not become NaN by a power that has left the range.
+__device__ __forceinline__ float decay_power(float log_decay, int n) {
+  return n == 0 ? 1.f : fmaxf(expf(log_decay * n), log_decay > -INFINITY ? 1.17549435e-38f : 0.f);
+}
 
 // ---------------------------------------------------------------- single tokens
 //
@@ -267,6 +270,13 @@ struct Split<bf16> {
       for (int i = 0; i < 4; ++i) x[i] -= __uint_as_float(__float_as_uint(x[i]) & 0xffff0000u);
     }
   }
+  // Infinities of x are their first parts; else nothing is left to change.  (For every split a tenth of a call's time.)
+  __device__ __forceinline__ void keep_infinities(f32x4 x) {
+#pragma unroll
+    for (int p = 1; p < parts; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[p][i] = fabsf(x[i]) == INFINITY ? 0 : part[p][i];
+  }
 };
 template <>
 struct Split<float> {
@@ -274,6 +284,7 @@ struct Split<float> {
   f32x4 part[1];
   static __device__ __forceinline__ f32x4 first(f32x4 x) { return x; }
   __device__ __forceinline__ explicit Split(f32x4 x) : part{x} {}
+  __device__ __forceinline__ void keep_infinities(f32x4) {}
 };
 
 // A tile of whole rows in LDS: piece p of row r lies at place p ^ swap(r) of it.
@@ -656,7 +667,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       }
     }
   };
-  auto update = [&](int buf, int n) {        // the state after a chunk of n tokens
+  auto update = [&](int buf, int n, bool infinities) {       // the state after a chunk of n tokens; infinities: V may hold some
     const char* const kb = k_lds + buf * Shape::q_bytes;
     const float an = power[n];
 #pragma unroll
@@ -670,7 +681,12 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       for (int y = 0; y < 2; ++y)
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[y][i] = left[C - n + summed<T>(j, y, g, i)];
-      const Split<T> v0(half_of(vt[j], 0) * w[0]), v1(half_of(vt[j], 1) * w[1]);
+      const f32x4 wv[2] = {half_of(vt[j], 0) * w[0], half_of(vt[j], 1) * w[1]};
+      Split<T> v0(wv[0]), v1(wv[1]);
+      if (infinities) {
+        v0.keep_infinities(wv[0]);
+        v1.keep_infinities(wv[1]);
+      }
 #pragma unroll
       for (int x0 = 0; x0 < KX; x0 += 2) {
         pair kd[2][2];
@@ -697,7 +713,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       if (more) load_kv(t + n, min(C, hi - t - n), kv ^ 1);
       if (columns) {
         read_v(kv, n);
-        update(kv, n);
+        update(kv, n, true);
       }
       if (!more) break;
       arrive<0>();
@@ -752,6 +768,16 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     constexpr bool HELD = DP <= 128 && PARTS > 1;
     pair sp[HELD ? KX : 1][PARTS];
     bool odd = false;                // whether one of the wave's values is not finite
+    bool infinite = false;           // whether its state holds infinities
+    auto split_state = [&](int to, int x) {
+      Split<T> s0(s[x][0]), s1(s[x][1]);
+      if (infinite) {
+        s0.keep_infinities(s[x][0]);
+        s1.keep_infinities(s[x][1]);
+      }
+#pragma unroll
+      for (int z = 1; z < PARTS; ++z) sp[to][z] = join(s0.part[z], s1.part[z]);
+    };
     bool stored = false;             // whether the last head's rows of out are known to be STORES stores of the wave
     arrive<0>();
     // (the state is here: else the compiler would wait for it, and for all that came after it, in every turn)
@@ -768,13 +794,19 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
 #pragma unroll
         for (int x = 0; x < CX; ++x) odd |= !all_finite(vt[x]);
         odd = __ballot(odd) != 0;
+        if (PARTS > 1) {
+          float top = 0.f;
+#pragma unroll
+          for (int x = 0; x < KX; ++x)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(s[x][y][i]));
+          infinite = __ballot(top == INFINITY) != 0;
+        }
         if (HELD) {
 #pragma unroll
-          for (int x = 0; x < KX; ++x) {
-            const Split<T> s0(s[x][0]), s1(s[x][1]);
-#pragma unroll
-            for (int z = 1; z < PARTS; ++z) sp[x][z] = join(s0.part[z], s1.part[z]);
-          }
+          for (int x = 0; x < KX; ++x) split_state(HELD ? x : 0, x);
         }
       }
       const char* const qt = q_lds + qb * Shape::q_bytes;
@@ -827,11 +859,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
             for (int ib = 0; ib < CT; ++ib) qf[(x + 1) & 1][ib] = operand(qt, q_at, 16 * ib, x + 1);
           }
           __builtin_amdgcn_sched_barrier(0);
-          if (!HELD) {
-            const Split<T> s0(s[x][0]), s1(s[x][1]);
-#pragma unroll
-            for (int z = 1; z < PARTS; ++z) sp[0][z] = join(s0.part[z], s1.part[z]);
-          }
+          if (!HELD) split_state(0, x);
           sp[HELD ? x : 0][0] = join(Split<T>::first(s[x][0]), Split<T>::first(s[x][1]));
 #pragma unroll
           for (int z = 0; z < PARTS; ++z)
@@ -840,7 +868,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
         }
 #pragma unroll
         for (int ib = 0; ib < CT; ++ib) o[ib] *= power[16 * ib + l16 + 1] * a.scale;
-        if (last && (t + n < hi || s_to)) update(kv, n);
+        if (last && (t + n < hi || s_to)) update(kv, n, odd);
       }
       // P is whole; the next head's Q and, after the last head, the next chunk's K and V are here: all that was asked for
       // but the last head's rows of out, which went off after it.  This head's Q and, after the last head, the chunk's K

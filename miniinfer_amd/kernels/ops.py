@@ -1242,7 +1242,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int,
   state as it is, rows of `out` that belong to no request are left as they are, and a state row outside the buffer gives
   rows of NaN.  log_decay float32 [nkv], <= 0 (-inf: a = 0) or positive for a growing state.  max_len: the most tokens of
   one request if the host knows it (default: T); it only chooses how the work is cut.  float32 and bfloat16; states and
-  sums are 32-bit."""
+  sums are 32-bit.  What is not finite makes what depends on it not finite and nothing else; infinities in states and in v
+  stay infinities in the state, where an infinite q or k may give NaN."""
   args = _linear_attention_call("linear_attention", q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay, scale,
                                 idle_row)
   _i32("cu_q", cu_q)
