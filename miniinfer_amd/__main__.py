@@ -16,6 +16,7 @@ import json
 import sys
 import time
 from random import Random
+from typing import Optional
 
 
 def _engine_args(p):
@@ -59,8 +60,22 @@ def _engine(args):
                    **({} if args.preset is not None else {"load_format": args.load_format}))
 
 
+def _beams_refused(args) -> Optional[str]:
+  """What is wrong with the options of a beam search, or None."""
+  from miniinfer_amd.kernels import ops
+  if not 0 <= args.beams <= ops.BEAM_MAX_COUNT // 2:
+    return f"--beams {args.beams}: 1 to {ops.BEAM_MAX_COUNT // 2} beams (0: no beam search)"
+  if args.beams and (args.temperature is not None or args.top_k != 0 or args.top_p != 1.0):
+    return "--beams searches for the most probable continuations: give no --temperature, --top-k or --top-p"
+  return None
+
+
 def cmd_generate(args) -> int:
   from miniinfer_amd import BeamSearchParams, SamplingParams
+  refused = _beams_refused(args)
+  if refused:
+    print(refused, file=sys.stderr)
+    return 2
   prompts = []
   for s in args.prompt or []:
     prompts.append(s)
@@ -75,9 +90,6 @@ def cmd_generate(args) -> int:
       print("give --prompt, --prompt-ids or --num-prompts", file=sys.stderr)
       return 2
     if args.beams:
-      if args.temperature is not None:
-        print("--beams searches for the most probable continuations: give no --temperature", file=sys.stderr)
-        return 2
       found = engine.beam_search(prompts, BeamSearchParams(num_beams=args.beams, max_tokens=args.max_tokens,
                                                            length_penalty=args.length_penalty, ignore_eos=args.ignore_eos))
       for p, hyps in zip(prompts, found):
