@@ -93,8 +93,11 @@ def cmd_generate(args) -> int:
       found = engine.beam_search(prompts, BeamSearchParams(num_beams=args.beams, max_tokens=args.max_tokens,
                                                            length_penalty=args.length_penalty, ignore_eos=args.ignore_eos))
       for p, hyps in zip(prompts, found):
-        print(json.dumps({"prompt": p, **hyps[0]}))
-      return 0
+        if hyps:
+          print(json.dumps({"prompt": p, **hyps[0]}))
+        else:
+          print(f"prompt {json.dumps(p)}: no continuation has a probability (logits of NaN or -inf only)", file=sys.stderr)
+      return 0 if all(found) else 1
     args.temperature = 0.7 if args.temperature is None else args.temperature
     sp = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                         ignore_eos=args.ignore_eos)

@@ -365,9 +365,10 @@ class LLMEngine:
   # ------------------------------------------------------------------ beam search
   def beam_search(self, prompts, params: Optional[BeamSearchParams] = None) -> List[List[dict]]:
     """The most probable continuations by beam search (prompts as in `generate`; not while other requests are unfinished).
-    Returns, for every prompt, its `num_return` best hypotheses as dicts with "text", "token_ids",
-    "cumulative_logprob", "score" (that over length ** length_penalty) and "finish_reason" ("eos", "stop" or
-    "length")."""
+    Returns, for every prompt, its `num_return` best hypotheses (fewer where fewer continuations have a probability above
+    zero, none where the logits are NaN) as dicts with "text", "token_ids", "cumulative_logprob", "score" (that over
+    length ** length_penalty) and "finish_reason" ("eos", "stop" or "length").  At most 32 beams, fewer where several tokens
+    end a hypothesis: a step's 64 candidates have to hold num_beams that go on whatever the others end with."""
     from .beam_search import BeamSearcher
     if isinstance(prompts, str) or (len(prompts) > 0 and isinstance(prompts[0], int)):
       prompts = [prompts]
