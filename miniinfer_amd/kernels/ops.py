@@ -1160,6 +1160,17 @@ def _linear_attention_rows(what, name, t, T, columns, dtype):
   return t.data_ptr(), stride[0]
 
 
+def _rows_meet(ap: int, astride: int, abytes: int, bp: int, bstride: int, bbytes: int, rows: int) -> bool:
+  """Whether two sets of `rows` rows of so many bytes share memory.  Rows of one wider buffer (equal strides) may lie between
+  one another; other sets count as sharing where their ranges cross."""
+  if ap + (rows - 1) * astride + abytes <= bp or bp + (rows - 1) * bstride + bbytes <= ap:
+    return False
+  if astride != bstride:
+    return True
+  at = (bp - ap) % astride                 # where b's rows begin in a's
+  return not abytes <= at <= astride - bbytes
+
+
 def _linear_attention_call(what, q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay, scale, idle_row):
   """The checked arguments of a launch, as its entry points take them."""
   if nkv < 1 or nq < nkv or nq % nkv:
@@ -1175,8 +1186,13 @@ def _linear_attention_call(what, q, k, v, nq, nkv, d, out, state, state_rows, cu
   op, os = _linear_attention_rows(what, "out", out, T, nqd, dtype)
   if out.shape[1] != nqd:
     raise KernelError(f"{what}: out {tuple(out.shape)} is not [{T}, {nqd}]")
-  if T and op in (qp, kp, vp):
-    raise KernelError(f"{what}: out shares memory with an input")
+  if T:
+    size = 2 if code == BF16 else 4
+    end = op + T * os * size
+    if (op < qp + T * qs * size and qp < end) or (op < kp + T * ks * size and kp < end) or (op < vp + T * vs * size and vp < end):
+      for p, s, n in ((qp, qs, nqd), (kp, ks, nkvd), (vp, vs, nkvd)):
+        if _rows_meet(op, os * size, nqd * size, p, s * size, n * size, T):
+          raise KernelError(f"{what}: out shares memory with an input")
   shape, stride, sp = state.shape, state.stride(), state.data_ptr()
   if state.dtype is not torch.float32 or len(shape) != 4 or shape[1:] != (nkv, d, d) or stride[2:] != (d, 1) \
       or (nkv > 1 and stride[1] != d * d):
