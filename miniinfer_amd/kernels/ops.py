@@ -1347,16 +1347,29 @@ MOVE_ROWS_MAX_BUFFERS = 8
 MOVE_ROWS_MAX = 16384        # moves of a call: one workgroup holds a piece of every moved row in its registers
 
 
+def _buffers_meet(a, b) -> bool:
+  """Whether two buffers of `move_rows` (address, bytes from layer to layer, from row to row and of a row, layers, rows)
+  share memory.  They do not where their ranges do not cross, nor where one lies between the layers or rows of the other
+  (parts of one larger tensor): where some stride, of which all wider ones are multiples, separates what they hold of a
+  period of it.  Anything else counts as sharing.  (For buffers whose ranges cross.)"""
+  axes = [[(s[i], s[i + 3]) for i in (1, 2) if s[i + 3] > 1] for s in (a, b)]
+  extent = lambda i, below: sum(st * (n - 1) for st, n in axes[i] if st < below) + (a, b)[i][3]
+  strides = {st for x in axes for st, _ in x}
+  return not any(extent(0, st) <= (b[0] - a[0]) % st <= st - extent(1, st) for st in strides
+                 if not any(wider % st for wider in strides if wider > st))
+
+
 def move_rows(buffers, src: torch.Tensor, dst: torch.Tensor) -> None:
   """In place, in every layer of every buffer: row dst[i] becomes what row src[i] was before the call, for all i as if
   at once (permutations and cycles are fine; a row may be a source more than once, a destination only once).  buffers: a
-  tensor or up to 8 of them that share no memory, [layers, rows, ...] with dense rows, of any dtype: a cache group's key
-  and value pages, a group's states.  src, dst: int32 [n] on the device, n up to 16,384; entries outside a buffer's rows move nothing there
-  (pad with -1)."""
+  tensor or up to 8 of them that share no memory (parts of one tensor are fine), [layers, rows, ...] with dense rows, of any
+  dtype: a cache group's key and value pages, a group's states.  src, dst: int32 [n] on the device, n up to 16,384; entries
+  outside a buffer's rows move nothing there (pad with -1)."""
   buffers = [buffers] if isinstance(buffers, torch.Tensor) else list(buffers)
   if not 1 <= len(buffers) <= MOVE_ROWS_MAX_BUFFERS:
     raise KernelError(f"move_rows: {len(buffers)} buffers, 1 to {MOVE_ROWS_MAX_BUFFERS} are taken")
   spec = []               # address, bytes from layer to layer, from row to row and of a row, layers, rows of each buffer
+  ranges = []             # the first byte of each and the one after its last
   for t in buffers:
     shape, total = t.shape, t.numel()
     if len(shape) < 2:
@@ -1377,9 +1390,15 @@ def move_rows(buffers, src: torch.Tensor, dst: torch.Tensor) -> None:
         extent += (n - 1) * stride
       per_layer = t.stride(0) if layers > 1 else row
       per_row = t.stride(1) if rows > 1 else row
-    spec += (t.data_ptr(), per_layer * size, per_row * size, row * size, layers, rows)
+    at = t.data_ptr()
+    spec += (at, per_layer * size, per_row * size, row * size, layers, rows)
+    ranges.append((at, at + (per_layer * (layers - 1) + per_row * (rows - 1) + row) * size))
   if len(set(spec[::6])) != len(spec) // 6:
     raise KernelError("move_rows: a buffer is given twice")
+  for i, (at, end) in enumerate(ranges):
+    for j, (other, other_end) in enumerate(ranges[:i]):
+      if at < other_end and other < end and _buffers_meet(spec[6 * j:6 * j + 6], spec[6 * i:6 * i + 6]):
+        raise KernelError("move_rows: buffers share memory")
   n = src.numel()
   if src.dtype is not torch.int32 or dst.dtype is not torch.int32 or not src.is_contiguous() or not dst.is_contiguous():
     _i32("src", src)

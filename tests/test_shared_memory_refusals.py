@@ -59,3 +59,60 @@ def test_an_out_after_the_parts_of_a_wider_buffer_is_taken():
   for call in _calls(q, k, v, out):
     with pytest.raises(KernelError, match="GPU only"):
       call()
+
+
+def _move(*buffers):
+  i = torch.zeros(1, dtype=torch.int32)
+  ops.move_rows(list(buffers), i, i)
+
+
+def _pairs():
+  t = torch.zeros(3, 8, 4, 6)
+  kv = torch.zeros(3, 2, 8, 4)                                   # [layers, keys and values, rows, ...]
+  by_row = torch.zeros(3, 8, 2, 4)                               # a row's keys, then its values
+  flat = torch.zeros(400)
+  for a, b in ((t, t[:, 1:]), (t, t[1:]), (t[:2], t[1:]), (t[:, :5], t[:, 4:]), (t[:, ::2], t[:, 2::2]), (t[:, ::3], t[:, 1::2]),
+               (flat[:80].view(2, 5, 8), flat[79:159].view(2, 5, 8)), (t[0:1], t[:, 3:4]), (by_row[:, :, 0, :3], by_row[:, :, 0, 2:]),
+               (kv[:, 0], kv[:, :, 1])):
+    yield a, b, True
+  for a, b in ((t[:1], t[1:]), (t[:, :5], t[:, 5:]), (t[:, ::2], t[:, 1::2]), (t[::2], t[1::2]), (kv[:, 0], kv[:, 1]),
+               (by_row[:, :, 0], by_row[:, :, 1]), (by_row[:, :, 0, :2], by_row[:, :, 0, 2:]),
+               (flat[:80].view(2, 5, 8), flat[80:160].view(2, 5, 8)), (t[:1, :1], t[1:2, 1:2]), (t[:, 0:1], t[:, 7:]),
+               (kv[:, 0].transpose(0, 1), kv[:, 1].transpose(0, 1))):
+    yield a, b, False
+
+
+@pytest.mark.parametrize("case", range(21))
+@pytest.mark.parametrize("turned", [False, True])
+def test_move_rows_refuses_buffers_that_share_memory(case, turned):
+  a, b, shares = list(_pairs())[case]
+  assert _shares(a, b) == shares
+  with pytest.raises(KernelError, match="share memory|twice" if shares else "GPU only"):
+    _move(*((b, a) if turned else (a, b)))
+  with pytest.raises(KernelError, match="share memory|twice" if shares else "GPU only"):
+    _move(torch.zeros(2, 3), a, torch.zeros(1, 4), b)
+
+
+def test_move_rows_takes_no_buffers_that_share_memory():
+  """Any two views of one buffer."""
+  import random
+  rng = random.Random(3)
+  flat = torch.zeros(600)
+  taken = refused = 0
+  for _ in range(4000):
+    views = []
+    for _ in range(2):
+      row, layers, rows = rng.randint(1, 5), rng.randint(1, 4), rng.randint(1, 5)
+      per_row = row + rng.choice([0, 0, 1, 3, 7])
+      per_layer = per_row * rows + rng.choice([0, 0, 1, 4, per_row])
+      if rng.random() < 0.3:
+        per_layer = row + rng.choice([0, 1, 3])
+        per_row = per_layer * layers + rng.choice([0, 2])
+      views.append(flat.as_strided((layers, rows, row), (per_layer, per_row, 1), rng.randint(0, 200)))
+    shares = _shares(*views)
+    with pytest.raises(KernelError) as e:
+      _move(*views)
+    if shares:
+      assert "share memory" in str(e.value) or "twice" in str(e.value)
+    taken, refused = taken + ("GPU only" in str(e.value)), refused + ("GPU only" not in str(e.value))
+  assert taken > 500 and refused > 500
