@@ -190,8 +190,8 @@ MI_EXPORT int mi_linear_attention_step(LA_ARGS, hipStream_t stream) {
 //
 // The bfloat16 form multiplies what is 32-bit (S, the weighted P and w V) as it is: split into three bfloat16 parts whose sum
 // it is to the last bit, one after the other into the same accumulators.  (Two parts for S and P leave out 2^-17 of a term,
-// which an output keeps where its terms cancel; they were 8 to 11% quicker, 32,768 tokens 227 us against 252.)  The one
-// rounding to fewer bits is the output's.
+// which an output keeps where its terms cancel.  They were 4 to 13% quicker: 2,048 tokens 31 us against 32, 24 ragged
+// requests 68 against 78, 32,768 tokens 233 against 260.)  The one rounding to fewer bits is the output's.
 //
 // Operands: lane l of an operand has row l % 16 and, of 32 elements of the summed axis, with g = l / 16: in bfloat16
 // (16x16x32) the 8 from 8 g on, in 32 bits (eight products 16x16x4) the 4 from 4 g on and the 4 from 16 + 4 g on.  Its
@@ -203,7 +203,8 @@ MI_EXPORT int mi_linear_attention_step(LA_ARGS, hipStream_t stream) {
 // piece of 16 bytes that a lane asks for is chosen such that piece p of row r lies at place p ^ swap(r): then the
 // operands' reads, 16 pieces at a time (lanes 0-3, 12-15 and 20-27, ...), and the transposing reads, 16 times 8 bytes of
 // 4 rows, meet no bank twice (with p ^ 2 (r mod 4), as good for the former alone, the LDS was busy twice as long, and
-// 32,768 tokens of 32 heads on 8 of 128 took 209 us instead of 198, without the kernels for segments).
+// 32,768 tokens of 32 heads on 8 of 128 took 209 us instead of 198, without the kernels for segments, with S and P in two
+// parts).
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -529,12 +530,13 @@ struct ChunkShape {
   }
 };
 
-// What bounds it (that workload, 186 us at 3.6 TB/s; the counters at 198): the matrix cores are busy for 30% of the time,
-// the vector ALUs and the LDS for about as long, memory for half of it.  With 8 waves on a compute unit, all that the
-// registers (256) and the LDS (128 KB) allow, the waits between a head's products are not covered: without loads and stores
-// it took 142 us, without stores 25 less, without any one of the products 0 to 17 less.  Chunks of 32 tokens are slower
-// with heads of 128 (258 us for the whole call, 234 with 64) and quicker with heads up to 64, where several workgroups
-// share a compute unit (8,192 tokens, 32 heads: 76 us, 114 with 64).
+// What bounds it (that workload, 214 us at 3.1 TB/s): the matrix cores are busy for 38% of the time, the vector ALUs and the
+// LDS for about as long, memory for half of it.  With 8 waves on a compute unit, all that the registers (256) and the LDS
+// (144 KB) allow, the waits between a head's products are not covered: with S and P in two parts it took 186 us, 142 of
+// them without loads and stores, 25 less without stores, 0 to 17 less without any one of the products.  Chunks of 32 tokens
+// are slower with heads of 128 (273 us for the whole call, 260 with 64; 8 requests of 8,192 tokens together 75, 70) and
+// were quicker with heads up to 64, where several workgroups share a compute unit (8,192 tokens, 32 heads: 76 us, 114 with
+// 64).
 //
 // STATES: only what a segment adds to its request's state (from zero), left in `work`; the last segment's is not needed.
 // ALIGNED: rows of q, k, v and out start at multiples of 16 bytes, and a chunk of a tensor spans less than 2^31 bytes.
@@ -812,7 +814,8 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
       const char* const qt = q_lds + qb * Shape::q_bytes;
       const char* const kt = k_lds + kv * Shape::q_bytes;
       char* const pt = p_lds + pb * Shape::p_bytes;
-      // ---- P^T.  All waves wait for it, so it goes before the other wave's products (32,768 tokens 229 us, without that 233)
+      // ---- P^T.  All waves wait for it, so it goes before the other wave's products (32,768 tokens 262 us, without that 264;
+      // 24 requests of 9,001 tokens together, 32 heads on 8, 164, 166)
       __builtin_amdgcn_s_setprio(1);
       if (block < BLOCKS) {
         f32x4 p[P_WIDE];

@@ -5,8 +5,8 @@
 //
 // A row may be a source and a destination in the same call (a permutation, cycles included): a workgroup owns a range
 // of columns of one layer for all of the call's moves, has every piece it reads in registers before it stores the
-// first one, and no other workgroup touches those columns.  So nothing is staged in memory: each source piece is read
-// once and each destination piece written once, which is what bounds the kernel.
+// first one, and no other workgroup touches those columns.  So nothing is staged in memory: a source piece is read for
+// each move that it is the source of, and each destination piece written once, which is what bounds the kernel.
 #include "common.h"
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -14,7 +14,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 #define ROWS_MAX_BUFFERS 8
 // Pieces that a thread holds.  Few of them, in workgroups of 512 threads, keep more workgroups on a compute unit, some
 // loading while others store (12 layers of 64 states of 512 KB: 146 us, 4.5 TB/s; with 16 pieces in 256 threads 174);
-// long lists take what registers there are, so that a row's columns still come in whole lines.
+// long lists take what registers there are, so that a row's columns come in whole lines for up to 2,048 moves (beyond,
+// pieces of a line to a workgroup, 16 bytes at 16,384).
 #define ROWS_PIECES 4
 #define ROWS_THREADS 512
 #define ROWS_PIECES_MANY 16

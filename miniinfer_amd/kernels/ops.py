@@ -1235,9 +1235,9 @@ def linear_attention_segment(num_tokens: int, num_requests: int, max_len: int, n
   """Tokens of a segment into which requests are cut, 0 for none: as many (whole chunks of 64) as make one workgroup for
   every compute unit over all tokens, two of the small ones of head sizes up to 64.  Every request's last segment may be a
   short one, and a workgroup too many is a second turn on its compute unit, so they are counted, up to half of all (8
-  requests of 8,192 tokens together, 8 heads of 128: 67 us in segments of 384, 89 in segments of 256).  A cut costs a pass
+  requests of 8,192 tokens together, 8 heads of 128: 73 us in segments of 384, 89 in segments of 256).  A cut costs a pass
   over the keys and values for the segments' states and a kernel that adds them up, so a longest request of up to two
-  segments is left whole (24 requests of up to 950 tokens, 12 heads of 80: 74 us whole, 93 in segments of 384)."""
+  segments is left whole (24 requests of up to 950 tokens, 12 heads of 80: 79 us whole, 91 in segments of 384)."""
   workgroups = _linear_attention_workgroups(nkv, d, itemsize, units)
   tokens = max(64, -(-num_tokens // (64 * max(1, workgroups - num_requests + 1, workgroups // 2))) * 64)
   return tokens if max_len > 2 * tokens else 0
@@ -1256,10 +1256,11 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, nq: int,
   idle_row: a row that stands for none; requests on it, any number, start from zeros and leave nothing (the padding
   entries of captured steps).  cu_q int32 [B + 1] = first token of each request: a request without tokens leaves its
   state as it is, rows of `out` that belong to no request are left as they are, and a state row outside the buffer gives
-  rows of NaN.  log_decay float32 [nkv], <= 0 (-inf: a = 0) or positive for a growing state.  max_len: the most tokens of
-  one request if the host knows it (default: T); it only chooses how the work is cut.  float32 and bfloat16; states and
-  sums are 32-bit.  What is not finite makes what depends on it not finite and nothing else; infinities in states and in v
-  stay infinities in the state, where an infinite q or k may give NaN."""
+  rows of NaN.  log_decay float32 [nkv], <= 0 (-inf: a = 0) or positive for a growing state (as long as a's powers over a
+  call's tokens stay in the range of 32 bits).  max_len: the most tokens of one request if the host knows it (default: T);
+  it only chooses how the work is cut.  float32 and bfloat16; states, sums and the factors of products are 32-bit.  What is
+  not finite makes what depends on it not finite and nothing else; infinities in states and in v stay infinities in the
+  state, where an infinite q or k may give NaN."""
   args = _linear_attention_call("linear_attention", q, k, v, nq, nkv, d, out, state, state_rows, cu_q, log_decay, scale,
                                 idle_row)
   _i32("cu_q", cu_q)
