@@ -18,7 +18,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // 0.4 * 2^-24 of the weight 1 for a decay.)  Only a decay of zero has powers of zero, the others end at the
 // smallest normal number: an infinity in a state or a value does not become NaN by a power that has left the range.
 __device__ __forceinline__ float decay_power(float log_decay, int n) {
-  return n == 0 ? 1.f : fmaxf(expf(log_decay * n), log_decay > -INFINITY ? 1.17549435e-38f : 0.f);
+  const float least = 1.17549435e-38f, power = n == 0 ? 1.f : expf(log_decay * n);
+  return power < least && log_decay > -INFINITY ? least : power;          // (of NaN NaN)
 }
 
 // ---------------------------------------------------------------- single tokens
