@@ -16,9 +16,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // a^n; a^0 = 1 for a decay of zero too.  (The product's rounding puts an error of |n log a| 2^-24 on the power, at most
 // 0.4 * 2^-24 of the weight 1 for a decay.)  Only a decay of zero has powers of zero, the others end at the
-// smallest normal number: an infinity in a state or a value does not become NaN by a power that has left the range.
+// smallest number: an infinity in a state or a value does not become NaN by a power that has left the range.
 __device__ __forceinline__ float decay_power(float log_decay, int n) {
-  const float least = 1.17549435e-38f, power = n == 0 ? 1.f : expf(log_decay * n);
+  const float least = 1.4e-45f, power = n == 0 ? 1.f : expf(log_decay * n);
   return power < least && log_decay > -INFINITY ? least : power;          // (of NaN NaN)
 }
 
@@ -253,7 +253,7 @@ __device__ __forceinline__ f32x4 widen(s16x4 h) {
 __device__ __forceinline__ f32x4 widen(f32x4 h) { return h; }
 
 // A 32-bit value as a sum of parts that the matrix cores take, exactly: a part is what is left cut off after 8 bits, and
-// 24 bits are three times 8.
+// 24 bits are three times 8.  (Bits below bfloat16's smallest number, 2^-133, are lost.)
 template <typename T>
 struct Split;
 template <>
@@ -549,6 +549,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
   constexpr int PARTS = Shape::parts, KX = DP / 32, KB = KX < 4 ? KX : 4, CX = C / 32, CT = C / 16, VS = Shape::VS;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   __shared__ float power[C + 1];     // a^i
+  __shared__ float scaled[C + 1];    // scale a^i, as far as it ends too
   __shared__ float left[2 * C];      // a^(C-1-i), zeros from C on
   __shared__ int found;
   char* const k_lds = lds;
@@ -608,6 +609,8 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
     if (tid <= C) {
       const float p = decay_power(a.log_decay[h], tid);
       power[tid] = p;
+      const float ps = p * a.scale;
+      scaled[tid] = ps == 0.f && p != 0.f && a.scale != 0.f ? copysignf(1.4e-45f, a.scale) : ps;
       if (tid < C) left[C - 1 - tid] = p;
     }
     for (int i = C + tid; i < 2 * C; i += Shape::threads) left[i] = 0.f;
@@ -765,7 +768,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
 #pragma unroll
     for (int w = 0; w < P_WIDE; ++w)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) weight[w][i] = power[min(max(reach - 16 * w - i, 0), C)] * a.scale;
+      for (int i = 0; i < 4; ++i) weight[w][i] = scaled[min(max(reach - 16 * w - i, 0), C)];
     // the state's parts but the first, which is the state's upper halves: held for all query heads of a chunk where there
     // are registers for them
     constexpr bool HELD = DP <= 128 && PARTS > 1;
@@ -871,7 +874,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void la_chunk_kernel(LinearAt
             for (int ib = 0; ib < CT; ++ib) mma(o[ib], sp[HELD ? x : 0][z], qf[x & 1][ib]);
         }
 #pragma unroll
-        for (int ib = 0; ib < CT; ++ib) o[ib] *= power[16 * ib + l16 + 1] * a.scale;
+        for (int ib = 0; ib < CT; ++ib) o[ib] *= scaled[16 * ib + l16 + 1];
         if (last && (t + n < hi || s_to)) update(kv, n, odd);
       }
       // P is whole; the next head's Q and, after the last head, the next chunk's K and V are here: all that was asked for
